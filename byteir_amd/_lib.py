@@ -94,18 +94,20 @@ def flash_attn():
         L = _load("libflash_attn.so", ctypes.RTLD_GLOBAL)
         vp = ctypes.c_void_p
         for n in ("run_flash_attn_fwd", "run_flash_attn_bwd", "run_flash_attn_fwd_bf16", "run_flash_attn_bwd_bf16",
-                  "run_flash_attn_kvcache", "run_flash_attn_kvcache_bf16"):
+                  "run_flash_attn_kvcache", "run_flash_attn_kvcache_bf16",
+                  *(f"run_flash_attn_{n}{t}" for n in ("sink_fwd", "sink_bwd", "paged", "evict") for t in ("", "_bf16"))):
             f = getattr(L, n)
             f.argtypes = [ctypes.POINTER(vp), vp, vp]
             f.restype = None
         sz, i32 = ctypes.c_size_t, ctypes.c_int
-        for n in ("fwd", "bwd", "kvcache"):
+        for n in ("fwd", "bwd", "kvcache", "sink_fwd", "sink_bwd", "paged", "evict"):
             getattr(L, f"flash_attn_{n}_checked").argtypes = [ctypes.POINTER(vp), vp, i32, vp]
             getattr(L, f"flash_attn_{n}_ws").argtypes = [ctypes.POINTER(vp), vp, i32, vp, sz, vp]
             getattr(L, f"flash_attn_{n}_workspace_bytes").restype = sz
-        L.flash_attn_fwd_workspace_bytes.argtypes = [vp, i32]
-        L.flash_attn_kvcache_workspace_bytes.argtypes = [vp, i32]
-        L.flash_attn_bwd_workspace_bytes.argtypes = [vp, i32, sz]
+        for n in ("fwd", "kvcache", "sink_fwd", "paged", "evict"):
+            getattr(L, f"flash_attn_{n}_workspace_bytes").argtypes = [vp, i32]
+        for n in ("bwd", "sink_bwd"):
+            getattr(L, f"flash_attn_{n}_workspace_bytes").argtypes = [vp, i32, sz]
         L.flash_attn_last_error.restype = ctypes.c_char_p
         _flash = L
     return _flash

@@ -244,19 +244,23 @@ public:
     // The (tensors, extra_args, stream) ABI has no error channel and no way to hand over
     // scratch: this library's plain entry points abort on arguments they cannot serve and
     // allocate their scratch themselves.  When the library also exports the extended forms
-    // (flash_attn_{fwd,bwd,kvcache}_ws + _workspace_bytes + flash_attn_last_error), the op kernel
+    // (flash_attn_{fwd,bwd,kvcache,sink_*,paged,evict}_ws + _workspace_bytes + flash_attn_last_error), the op kernel
     // uses those: a bad module fails Session::Run instead of ending the process, and the
     // scratch is a per-frame workspace from the frame's allocator, sized when the frame is set up.
     static const struct { const char *api, *stem; int dtype; } kExtended[] = {
         {"run_flash_attn_fwd", "flash_attn_fwd", 1},         {"run_flash_attn_fwd_bf16", "flash_attn_fwd", 2},
         {"run_flash_attn_bwd", "flash_attn_bwd", 1},         {"run_flash_attn_bwd_bf16", "flash_attn_bwd", 2},
-        {"run_flash_attn_kvcache", "flash_attn_kvcache", 1}, {"run_flash_attn_kvcache_bf16", "flash_attn_kvcache", 2}};
+        {"run_flash_attn_kvcache", "flash_attn_kvcache", 1}, {"run_flash_attn_kvcache_bf16", "flash_attn_kvcache", 2},
+        {"run_flash_attn_sink_fwd", "flash_attn_sink_fwd", 1}, {"run_flash_attn_sink_fwd_bf16", "flash_attn_sink_fwd", 2},
+        {"run_flash_attn_sink_bwd", "flash_attn_sink_bwd", 1}, {"run_flash_attn_sink_bwd_bf16", "flash_attn_sink_bwd", 2},
+        {"run_flash_attn_paged", "flash_attn_paged", 1},       {"run_flash_attn_paged_bf16", "flash_attn_paged", 2},
+        {"run_flash_attn_evict", "flash_attn_evict", 1},       {"run_flash_attn_evict_bf16", "flash_attn_evict", 2}};
     for (const auto &c : kExtended) {
       if (api_name != c.api) continue;
       const std::string stem(c.stem);
       with_ws_ = reinterpret_cast<WsFn>(dlsym(handle_, (stem + "_ws").c_str()));
       last_error_ = reinterpret_cast<LastErrorFn>(dlsym(handle_, "flash_attn_last_error"));
-      is_bwd_ = stem == "flash_attn_bwd";
+      is_bwd_ = stem == "flash_attn_bwd" || stem == "flash_attn_sink_bwd";
       if (is_bwd_) bwd_bytes_ = reinterpret_cast<BwdBytesFn>(dlsym(handle_, (stem + "_workspace_bytes").c_str()));
       else bytes_ = reinterpret_cast<BytesFn>(dlsym(handle_, (stem + "_workspace_bytes").c_str()));
       ext_dtype_ = c.dtype;

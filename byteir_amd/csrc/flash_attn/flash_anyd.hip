@@ -20,6 +20,8 @@
 // (lib/dropout.h, lib/philox.cuh), evaluated here for the elements a lane holds in the MFMA
 // accumulator layout; the scalings follow the reference (forward: row sums of the undropped P,
 // O / p_keep; backward: D * p_keep, dS = P * (keep ? dP - D : -D), dQ and dK / p_keep, dV / p_keep).
+#include <climits>
+
 #include "flash_common.h"
 
 namespace fa {
@@ -37,12 +39,13 @@ struct AnyTileLoader {
   static constexpr int RPP = 256 / CPR;
   static constexpr int NP = (ROWS + RPP - 1) / RPP;
   uint4 reg[NP];
-  __device__ __forceinline__ void gload(const T *base, int64_t row_stride, int row0, int n_rows, int d) {
+  // with sinks: only rows from row_lo on or below `sink` are read, the others arrive as zeros
+  __device__ __forceinline__ void gload(const T *base, int64_t row_stride, int row0, int n_rows, int d, int row_lo = INT_MIN, int sink = 0) {
     const int c = threadIdx.x % CPR, r = threadIdx.x / CPR;
 #pragma unroll
     for (int s = 0; s < NP; ++s) {
       const int row = row0 + s * RPP + r;
-      if (r < RPP && s * RPP + r < ROWS && row < n_rows && c * 8 < d)
+      if (r < RPP && s * RPP + r < ROWS && row < n_rows && c * 8 < d && (row >= row_lo || row < sink))
         reg[s] = *reinterpret_cast<const uint4 *>(base + (int64_t)row * row_stride + c * 8);
       else
         reg[s] = uint4{0, 0, 0, 0};
@@ -185,7 +188,8 @@ __device__ __forceinline__ void block_of(const Params &p, int n_blocks, bool rev
 }
 
 // ---- forward ----------------------------------------------------------------------------------
-template <typename T, int DR, bool Drop>
+// Sink: as in flash_fwd.hip, the tiles of the sinks before those of the window
+template <typename T, int DR, bool Drop, bool Sink = false>
 __global__ void __launch_bounds__(256, DR <= 128 ? 2 : 1) fwd_anyd_kernel(const Params p) {
   using vec8 = typename Traits<T>::vec8;
   constexpr int KS = Pad<DR>::kPlain, VS = Pad<DR>::kTr;
@@ -208,8 +212,11 @@ __global__ void __launch_bounds__(256, DR <= 128 ? 2 : 1) fwd_anyd_kernel(const 
   row_limits_sk(p, sk, wq0 + 31, w_lo_last, w_hi_last);
   row_limits_sk(p, sk, m0, b_lo, t0);
   row_limits_sk(p, sk, m0 + kRows - 1, t1, b_hi);
-  const int n_min = b_lo / kTile;
-  const int n_max = b_hi > 0 ? (b_hi + kTile - 1) / kTile : 0;
+  idx::SinkTiles st{};
+  if constexpr (Sink) st = idx::sink_tile_range(p.sq, sk, p.wl, p.wr, p.n_sink, m0, kRows, kTile);
+  const int n_min = Sink ? 0 : b_lo / kTile;
+  const int n_max = Sink ? st.n : b_hi > 0 ? (b_hi + kTile - 1) / kTile : 0;
+  auto tile_kv0 = [&](int t) { return (Sink ? idx::sink_tile(st, t) : t) * kTile; };  // first key of the t-th tile
 
   const T *qg = static_cast<const T *>(p.q) + bi * p.q_bs + (int64_t)qrow * p.q_rs + hi * p.q_hs;
   const T *kg = static_cast<const T *>(p.k) + bi * p.k_bs + hk * p.k_hs;
@@ -221,6 +228,11 @@ __global__ void __launch_bounds__(256, DR <= 128 ? 2 : 1) fwd_anyd_kernel(const 
 
   AnyTileLoader<T, DR, kTile> lk, lv;
   auto gload = [&](int t) {
+    if constexpr (Sink) {
+      lk.gload(kg, p.k_rs, tile_kv0(t), st.hi, p.d, st.lo, st.sink);
+      lv.gload(vg, p.v_rs, tile_kv0(t), st.hi, p.d, st.lo, st.sink);
+      return;
+    }
     lk.gload(kg, p.k_rs, t * kTile, sk, p.d);
     lv.gload(vg, p.v_rs, t * kTile, sk, p.d);  // zero rows: 0 * finite stays finite in P V
   };
@@ -240,7 +252,7 @@ __global__ void __launch_bounds__(256, DR <= 128 ? 2 : 1) fwd_anyd_kernel(const 
     __syncthreads();
   }
   for (int t = n_min; t < n_max; ++t) {
-    const int kv0 = t * kTile;
+    const int kv0 = Sink ? tile_kv0(t) : t * kTile;
     if constexpr (kPrefetch) {
       if (t + 1 < n_max) gload(t + 1);
     } else {
@@ -249,7 +261,7 @@ __global__ void __launch_bounds__(256, DR <= 128 ? 2 : 1) fwd_anyd_kernel(const 
       __syncthreads();
     }
     // the wave sees nothing of this tile when it lies wholly outside the widest row window
-    const bool skip = kv0 >= w_hi_last || kv0 + kTile <= w_lo_first;
+    const bool skip = kv0 >= w_hi_last || (kv0 + kTile <= w_lo_first && !(Sink && kv0 < p.n_sink));
     if (!skip) {
       float16v s[2];
 #pragma unroll
@@ -261,13 +273,13 @@ __global__ void __launch_bounds__(256, DR <= 128 ? 2 : 1) fwd_anyd_kernel(const 
           s[kvb] = Traits<T>::mfma(a, qf[ks], s[kvb]);
         }
       }
-      if (kv0 + kTile > w_hi_first || kv0 < w_lo_last) {  // a tile on the edge of the window
+      if (kv0 + kTile > w_hi_first || (kv0 < w_lo_last && !(Sink && kv0 + kTile <= p.n_sink))) {  // a tile on the edge of the window
 #pragma unroll
         for (int kvb = 0; kvb < 2; ++kvb)
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             const int kv = kv0 + kvb * 32 + (i >> 2) * 8 + g * 4 + (i & 3);
-            if (kv >= hi_lim || kv < lo_lim) s[kvb][i] = -INFINITY;
+            if (kv >= hi_lim || (kv < lo_lim && !(Sink && kv < p.n_sink))) s[kvb][i] = -INFINITY;
           }
       }
       float mx = -INFINITY;
@@ -398,8 +410,8 @@ __global__ void __launch_bounds__(256, DR <= 64 ? 2 : 1) dkdv_anyd_kernel(const 
   vec8 kf[DR / 16], vf[DR / 16];
 #pragma unroll
   for (int ks = 0; ks < DR / 16; ++ks) {
-    kf[ks] = load_frag<T>(kg, kvcol < p.sk, ks * 16 + g * 8, p.d);
-    vf[ks] = load_frag<T>(vg, kvcol < p.sk, ks * 16 + g * 8, p.d);
+    kf[ks] = load_frag<T>(kg, kvcol < p.kv_hi && kvcol >= p.kv_lo, ks * 16 + g * 8, p.d);
+    vf[ks] = load_frag<T>(vg, kvcol < p.kv_hi && kvcol >= p.kv_lo, ks * 16 + g * 8, p.d);
   }
   float16v dk_acc[DR / 32], dv_acc[DR / 32];
 #pragma unroll
@@ -537,7 +549,7 @@ __global__ void __launch_bounds__(256, DR <= 64 ? 2 : 1) dkdv_anyd_kernel(const 
 }
 
 // ---- backward 3: dQ ---------------------------------------------------------------------------------
-template <typename T, int DR, bool Drop>
+template <typename T, int DR, bool Drop, bool Sink = false>
 __global__ void __launch_bounds__(256, (DR <= 96 || (DR == 128 && !Drop)) ? 2 : 1) dq_anyd_kernel(const Params p) {
   using vec8 = typename Traits<T>::vec8;
   constexpr int KS = Pad<DR>::kPlain;  // K tile: plain and transposed reads
@@ -559,8 +571,11 @@ __global__ void __launch_bounds__(256, (DR <= 96 || (DR == 128 && !Drop)) ? 2 : 
   row_limits(p, wq0 + 31, w_lo_last, w_hi_last);
   row_limits(p, m0, b_lo, t0);
   row_limits(p, m0 + kRows - 1, t1, b_hi);
-  const int n_min = b_lo / kTile;
-  const int n_max = b_hi > 0 ? (b_hi + kTile - 1) / kTile : 0;
+  idx::SinkTiles st{};
+  if constexpr (Sink) st = idx::sink_tile_range(p.sq, p.sk, p.wl, p.wr, p.n_sink, m0, kRows, kTile);
+  const int n_min = Sink ? 0 : b_lo / kTile;
+  const int n_max = Sink ? st.n : b_hi > 0 ? (b_hi + kTile - 1) / kTile : 0;
+  auto tile_kv0 = [&](int t) { return (Sink ? idx::sink_tile(st, t) : t) * kTile; };  // first key of the t-th tile
 
   const T *qg = static_cast<const T *>(p.q) + bi * p.q_bs + (int64_t)qrow * p.q_rs + hi * p.q_hs;
   const T *dog = static_cast<const T *>(p.dout) + bi * p.o_bs + (int64_t)qrow * p.o_rs + hi * p.o_hs;
@@ -588,6 +603,11 @@ __global__ void __launch_bounds__(256, (DR <= 96 || (DR == 128 && !Drop)) ? 2 : 
 
   AnyTileLoader<T, DR, kTile> lk, lv;
   auto gload = [&](int t) {
+    if constexpr (Sink) {
+      lk.gload(kg, p.k_rs, tile_kv0(t), st.hi, p.d, st.lo, st.sink);
+      lv.gload(vg, p.v_rs, tile_kv0(t), st.hi, p.d, st.lo, st.sink);
+      return;
+    }
     lk.gload(kg, p.k_rs, t * kTile, p.sk, p.d);
     lv.gload(vg, p.v_rs, t * kTile, p.sk, p.d);
   };
@@ -599,7 +619,7 @@ __global__ void __launch_bounds__(256, (DR <= 96 || (DR == 128 && !Drop)) ? 2 : 
     __syncthreads();
   }
   for (int t = n_min; t < n_max; ++t) {
-    const int kv0 = t * kTile;
+    const int kv0 = Sink ? tile_kv0(t) : t * kTile;
     if constexpr (kPrefetch) {
       if (t + 1 < n_max) gload(t + 1);
     } else {
@@ -607,9 +627,9 @@ __global__ void __launch_bounds__(256, (DR <= 96 || (DR == 128 && !Drop)) ? 2 : 
       lstore();
       __syncthreads();
     }
-    const bool skip = kv0 >= w_hi_last || kv0 + kTile <= w_lo_first;
+    const bool skip = kv0 >= w_hi_last || (kv0 + kTile <= w_lo_first && !(Sink && kv0 < p.n_sink));
     if (!skip) {
-      const bool need_mask = kv0 + kTile > w_hi_first || kv0 < w_lo_last;
+      const bool need_mask = kv0 + kTile > w_hi_first || (kv0 < w_lo_last && !(Sink && kv0 + kTile <= p.n_sink));
       float16v s[2], dp[2];
 #pragma unroll
       for (int kvb = 0; kvb < 2; ++kvb) {
@@ -632,7 +652,7 @@ __global__ void __launch_bounds__(256, (DR <= 96 || (DR == 128 && !Drop)) ? 2 : 
           float pe = exp2_fast(fmaf(s[kvb][i], c, -lse_l));
           if (need_mask) {
             const int kv = kv0 + kvb * 32 + (i >> 2) * 8 + g * 4 + (i & 3);
-            if (kv >= hi_lim || kv < lo_lim) pe = 0.f;
+            if (kv >= hi_lim || (kv < lo_lim && !(Sink && kv < p.n_sink))) pe = 0.f;
           }
           const bool kept = !Drop || ((keep >> i) & 1u);
           s[kvb][i] = pe * ((kept ? dp[kvb][i] : 0.f) - dsm_l);  // dS^T
@@ -669,7 +689,8 @@ __global__ void __launch_bounds__(256, (DR <= 96 || (DR == 128 && !Drop)) ? 2 : 
 template <typename T, int DR>
 hipError_t fwd_anyd_d(const Params &p, hipStream_t stream) {
   const dim3 grid((unsigned)(p.n_mblocks * p.b * p.h)), block(256);
-  if (p.drop) FA_LAUNCH((fwd_anyd_kernel<T, DR, true>), grid, block, stream, p);
+  if (p.sink) FA_LAUNCH((fwd_anyd_kernel<T, DR, false, true>), grid, block, stream, p);
+  else if (p.drop) FA_LAUNCH((fwd_anyd_kernel<T, DR, true>), grid, block, stream, p);
   else FA_LAUNCH((fwd_anyd_kernel<T, DR, false>), grid, block, stream, p);
   return hipGetLastError();
 }
@@ -695,7 +716,8 @@ hipError_t bwd_anyd_d(const Params &p, hipStream_t stream) {
     }
   }
   if (p.n_mblocks > 0 && !p.ws_query) {
-    if (p.drop) FA_LAUNCH((dq_anyd_kernel<T, DR, true>), gq, block, stream, p);
+    if (p.sink) FA_LAUNCH((dq_anyd_kernel<T, DR, false, true>), gq, block, stream, p);
+    else if (p.drop) FA_LAUNCH((dq_anyd_kernel<T, DR, true>), gq, block, stream, p);
     else FA_LAUNCH((dq_anyd_kernel<T, DR, false>), gq, block, stream, p);
   }
   return hipGetLastError();
@@ -741,7 +763,10 @@ hipError_t launch_dq_anyd128(const Params &p, int dtype, hipStream_t stream) {
   pq.n_mblocks = (p.sq + kRows - 1) / kRows;
   if (pq.n_mblocks == 0) return hipSuccess;
   const dim3 grid((unsigned)(pq.n_mblocks * p.b * p.h)), block(256);
-  if (dtype == 1) FA_LAUNCH((dq_anyd_kernel<_Float16, 128, false>), grid, block, stream, pq);
+  if (p.sink) {
+    if (dtype == 1) FA_LAUNCH((dq_anyd_kernel<_Float16, 128, false, true>), grid, block, stream, pq);
+    else FA_LAUNCH((dq_anyd_kernel<__bf16, 128, false, true>), grid, block, stream, pq);
+  } else if (dtype == 1) FA_LAUNCH((dq_anyd_kernel<_Float16, 128, false>), grid, block, stream, pq);
   else FA_LAUNCH((dq_anyd_kernel<__bf16, 128, false>), grid, block, stream, pq);
   return hipGetLastError();
 }

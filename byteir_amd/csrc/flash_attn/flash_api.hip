@@ -12,6 +12,7 @@
 
 #include "flash_api.h"
 #include "flash_common.h"
+#include "flash_paged.h"
 
 namespace fa {
 hipError_t launch_fwd(Params &p, int dtype, hipStream_t stream);
@@ -126,6 +127,29 @@ KvBlob parse_kv(const void *extra_args) {
   return a;
 }
 
+// Sequential reader of an unpadded blob.
+struct Reader {
+  const unsigned char *s;
+  int64_t i64() { int64_t v; memcpy(&v, s, 8); s += 8; return v; }
+  float f32() { float v; memcpy(&v, s, 4); s += 4; return v; }
+};
+
+// extra_args of flash_attn_sink_{fwd,bwd}: the forward blob (192 bytes), then n_sink
+int sink_args(const void *extra_args, const Blob &a, fa::Params &p) {
+  Reader r{static_cast<const unsigned char *>(extra_args) + 192};
+  const int64_t n_sink = r.i64();
+  if (n_sink < 0) return fail("n_sink %ld is negative", (long)n_sink);
+  if (p.drop) return fail("dropout is not supported with sinks");
+  if (!(a.softmax_scale > 0.f) || std::isinf(a.softmax_scale)) return fail("softmax_scale %g is not positive and finite", a.softmax_scale);
+  if (a.b * a.h_k * ((n_sink < a.seqlen_k ? n_sink : a.seqlen_k) / 32 + 1) > (1 << 22)) return fail("problem too large for 32-bit tile indices");
+  p.sink = 1;
+  p.n_sink = (int)(n_sink < a.seqlen_k ? n_sink : a.seqlen_k);
+  // a window wider than the keys is no window; this also keeps row + window inside 32 bits
+  if (a.window_size_left >= a.seqlen_k + a.seqlen_q) p.wl = -1;
+  if (a.window_size_right >= a.seqlen_k + a.seqlen_q) p.wr = -1;
+  return 0;
+}
+
 }  // namespace
 
 extern "C" {
@@ -141,12 +165,14 @@ namespace {
 // *query receives the scratch the same call would take.
 struct Scratch { void *ws; size_t ws_bytes; size_t *query; };
 
-int fwd_impl(void **tensors, const void *extra_args, int dtype, const Scratch &sc, void *stream) {
+int fwd_impl(void **tensors, const void *extra_args, int dtype, const Scratch &sc, void *stream, bool sink = false) {
   if ((!tensors && !sc.query) || !extra_args) return fail("null argument");
   if (dtype != 1 && dtype != 2) return fail("dtype %d is not supported (1 = fp16, 2 = bf16)", dtype);
   const Blob a = parse(extra_args);
   fa::Params p{};
   if (int r = fill(a, p)) return r;
+  if (sink)
+    if (int r = sink_args(extra_args, a, p)) return r;
   p.ws = sc.ws; p.ws_bytes = sc.ws_bytes; p.ws_query = sc.query;
   if (sc.query) {
     *sc.query = 0;
@@ -166,12 +192,14 @@ int fwd_impl(void **tensors, const void *extra_args, int dtype, const Scratch &s
 }
 
 // dq_accum_bytes: only read when planning (the size of the dq_accum tensor the call will get)
-int bwd_impl(void **tensors, const void *extra_args, int dtype, const Scratch &sc, size_t dq_accum_bytes, void *stream) {
+int bwd_impl(void **tensors, const void *extra_args, int dtype, const Scratch &sc, size_t dq_accum_bytes, void *stream, bool sink = false) {
   if ((!tensors && !sc.query) || !extra_args) return fail("null argument");
   if (dtype != 1 && dtype != 2) return fail("dtype %d is not supported (1 = fp16, 2 = bf16)", dtype);
   const Blob a = parse(extra_args);
   fa::Params p{};
   if (int r = fill(a, p)) return r;
+  if (sink)
+    if (int r = sink_args(extra_args, a, p)) return r;
   if (a.seqlen_q_rounded < a.seqlen_q) return fail("seqlen_q_rounded < seqlen_q");
   p.ws = sc.ws; p.ws_bytes = sc.ws_bytes; p.ws_query = sc.query;
   if (sc.query) {
@@ -254,9 +282,185 @@ int kvcache_impl(void **tensors, const void *extra_args, int dtype, const Scratc
   return fa::launch_fwd(p, dtype, stream);
 }
 
+int page_args(fa::Pages &g, const char *what, int64_t num_pages, int64_t page, int64_t max_pages, int64_t b) {
+  if (num_pages < 0 || num_pages > INT32_MAX || page <= 0 || max_pages < 0) return fail("%s: bad page counts (%ld pages of %ld rows, %ld in a table row)", what, (long)num_pages, (long)page, (long)max_pages);
+  if (page > (1 << 30) || max_pages > (1 << 30) || (max_pages ? max_pages : 1) * page > (1 << 30)) return fail("%s: more than 2^30 rows in a sequence", what);
+  if (max_pages == 0 && num_pages < b) return fail("%s: %ld sequences in a cache of %ld", what, (long)b, (long)num_pages);
+  g.num_pages = (int)num_pages;
+  g.max_pages = (int)max_pages;
+  fa::set_page(g, (int)page);
+  return 0;
+}
+
+int heads_args(int64_t b, int64_t h, int64_t h_k, int64_t d) {
+  if (b < 0 || h <= 0 || h_k <= 0) return fail("negative or zero dimension (b=%ld h=%ld h_k=%ld)", (long)b, (long)h, (long)h_k);
+  if (d <= 0 || d > 256 || d % 8 != 0) return fail("head_dim %ld is not supported (a multiple of 8 up to 256)", (long)d);
+  if (h % h_k != 0) return fail("h (%ld) must be a multiple of h_k (%ld)", (long)h, (long)h_k);
+  if (b > (1 << 24) || h > (1 << 24) || b * h > (1 << 24)) return fail("problem too large for 32-bit tile indices");
+  return 0;
+}
+
+int stride_args(const int64_t *strides, int n) {
+  for (int i = 0; i < n; ++i)
+    if (strides[i] % 8 != 0) return fail("stride %ld is not a multiple of 8 elements (16-byte rows needed)", (long)strides[i]);
+  return 0;
+}
+
+// extra_args of flash_attn_paged: see flash_api.h
+int paged_impl(void **tensors, const void *extra_args, int dtype, const Scratch &sc, void *stream) {
+  if ((!tensors && !sc.query) || !extra_args) return fail("null argument");
+  if (dtype != 1 && dtype != 2) return fail("dtype %d is not supported (1 = fp16, 2 = bf16)", dtype);
+  Reader r{static_cast<const unsigned char *>(extra_args)};
+  int64_t st[18];
+  for (int64_t &x : st) x = r.i64();
+  const int64_t b = r.i64(), h = r.i64(), h_k = r.i64(), d = r.i64(), n_new = r.i64();
+  const float scale = r.f32();
+  const int64_t sq = r.i64(), num_pages = r.i64(), page = r.i64(), max_pages = r.i64();
+  const int64_t wl = r.i64(), wr = r.i64(), n_sink = r.i64(), weights = r.i64();
+  if (int e = heads_args(b, h, h_k, d)) return e;
+  if (int e = stride_args(st, 18)) return e;
+  fa::PagedParams p{};
+  if (int e = page_args(p.pages, "cache", num_pages, page, max_pages, b)) return e;
+  if (sq < 0 || n_new < 0 || sq > (1 << 30) || n_new > (1 << 30)) return fail("bad seqlen_q %ld or seqlen_knew %ld", (long)sq, (long)n_new);
+  if (n_sink < 0) return fail("n_sink %ld is negative", (long)n_sink);
+  if (weights < 0 || weights > 2) return fail("weights mode %ld is not 0, 1 or 2", (long)weights);
+  if (!(scale > 0.f) || std::isinf(scale)) return fail("softmax_scale %g is not positive and finite", scale);
+  const int64_t cap = p.pages.capacity();
+  p.q_bs = st[0]; p.pages.k_ps = st[1]; p.pages.v_ps = st[2]; p.kn_bs = st[3]; p.vn_bs = st[4]; p.o_bs = st[5];
+  p.q_rs = st[6]; p.pages.k_rs = st[7]; p.pages.v_rs = st[8]; p.kn_rs = st[9]; p.vn_rs = st[10]; p.o_rs = st[11];
+  p.q_hs = st[12]; p.pages.k_hs = st[13]; p.pages.v_hs = st[14]; p.kn_hs = st[15]; p.vn_hs = st[16]; p.o_hs = st[17];
+  p.b = (int)b; p.h = (int)h; p.h_k = (int)h_k; p.d = (int)d; p.sq = (int)sq; p.n_new = (int)n_new;
+  p.scale = scale;
+  p.scale_log2 = (float)(scale * M_LOG2E);
+  // a window wider than everything is no window
+  p.wl = wl < 0 || wl >= cap + sq ? -1 : (int)wl;
+  p.wr = wr < 0 || wr >= cap + sq ? -1 : (int)wr;
+  p.n_sink = (int)(n_sink < cap ? n_sink : cap);
+  p.ws = sc.ws; p.ws_bytes = sc.ws_bytes; p.ws_query = sc.query;
+  // the threads of a launch are counted in 32 bits
+  const int64_t tiles = b * h_k * ((h / h_k * sq + 31) / 32);
+  if (h / h_k * sq > (1 << 30) || tiles > (1 << 22) || b * h * sq > (1 << 30) || b * h_k * n_new > (1ll << 31) / (d / 8) || b * h_k * (cap / 256 + 1) > (1 << 23))
+    return fail("problem too large for 32-bit tile indices");
+  if (sc.query) *sc.query = 0;
+  if (b == 0 || sq == 0) {  // nothing attends; new rows are still appended
+    if (b == 0 || n_new == 0 || sc.query) return 0;
+    return fail("new rows without query rows (seqlen_q 0, seqlen_knew %ld)", (long)n_new);
+  }
+  if (sc.query) {
+    static float any;  // only whether there are weights matters when planning
+    p.w_out = weights ? &any : nullptr;
+    return fa::launch_paged(p, dtype, nullptr);
+  }
+  // tensors: q, k_pages, v_pages, k_new, v_new, block_table, seqlens_k, o, softmax_lse, weights, weights_out
+  p.q = tensors[0]; p.k = tensors[1]; p.v = tensors[2];
+  if (n_new) { p.k_new = tensors[3]; p.v_new = tensors[4]; }
+  if (max_pages) p.pages.table = static_cast<const int *>(tensors[5]);
+  p.seqlens = static_cast<const int *>(tensors[6]);
+  p.o = tensors[7];
+  p.lse = static_cast<float *>(tensors[8]);
+  if (weights == 2) p.w_in = static_cast<const float *>(tensors[9]);
+  if (weights) p.w_out = static_cast<float *>(tensors[10]);
+  if (!p.q || !p.seqlens || !p.o || !p.lse || (num_pages > 0 && (!p.k || !p.v)) || (n_new && (!p.k_new || !p.v_new)) || (max_pages && !p.pages.table) ||
+      (weights == 2 && !p.w_in) || (weights && !p.w_out))
+    return fail("null tensor pointer");
+  if (!aligned16(p.q) || !aligned16(p.k) || !aligned16(p.v) || !aligned16(p.o) || !aligned16(p.k_new) || !aligned16(p.v_new))
+    return fail("q, o, the caches and the new rows must be 16-byte aligned");
+  return fa::launch_paged(p, dtype, static_cast<hipStream_t>(stream));
+}
+
+// extra_args of flash_attn_evict: see flash_api.h.  It takes no scratch.
+int evict_impl(void **tensors, const void *extra_args, int dtype, const Scratch &sc, void *stream) {
+  if ((!tensors && !sc.query) || !extra_args) return fail("null argument");
+  if (dtype != 1 && dtype != 2) return fail("dtype %d is not supported (1 = fp16, 2 = bf16)", dtype);
+  Reader r{static_cast<const unsigned char *>(extra_args)};
+  int64_t st[12];
+  for (int64_t &x : st) x = r.i64();
+  const int64_t b = r.i64(), h_k = r.i64(), d = r.i64();
+  const int64_t np = r.i64(), page = r.i64(), mp = r.i64(), np_out = r.i64(), page_out = r.i64(), mp_out = r.i64();
+  const int64_t budget = r.i64(), n_sink = r.i64(), n_recent = r.i64();
+  if (int e = heads_args(b, h_k, h_k, d)) return e;
+  if (int e = stride_args(st, 12)) return e;
+  fa::EvictParams p{};
+  if (int e = page_args(p.from, "cache", np, page, mp, b)) return e;
+  if (int e = page_args(p.to, "output cache", np_out, page_out, mp_out, b)) return e;
+  if (budget <= 0 || budget > p.to.capacity()) return fail("budget %ld does not fit the output cache (%d rows a sequence)", (long)budget, p.to.capacity());
+  if (n_sink < 0 || n_recent < 0 || n_sink > budget || n_recent > budget - n_sink)
+    return fail("n_sink %ld and n_recent %ld do not fit the budget %ld", (long)n_sink, (long)n_recent, (long)budget);
+  if (b * h_k > (1ll << 31) / (budget * (d / 8 + 1))) return fail("problem too large for 32-bit tile indices");
+  if (sc.query) { *sc.query = 0; return 0; }
+  if (b == 0) return 0;
+  p.from.k_ps = st[0]; p.from.v_ps = st[1]; p.to.k_ps = st[2]; p.to.v_ps = st[3];
+  p.from.k_rs = st[4]; p.from.v_rs = st[5]; p.to.k_rs = st[6]; p.to.v_rs = st[7];
+  p.from.k_hs = st[8]; p.from.v_hs = st[9]; p.to.k_hs = st[10]; p.to.v_hs = st[11];
+  p.b = (int)b; p.h_k = (int)h_k; p.d = (int)d; p.budget = (int)budget; p.n_sink = (int)n_sink; p.n_recent = (int)n_recent;
+  // tensors: k, v, weights, seqlens_k, block_table, k_out, v_out, out_table, weights_out, seqlens_out, kept
+  p.k = tensors[0]; p.v = tensors[1];
+  p.w = static_cast<const float *>(tensors[2]);
+  p.seqlens = static_cast<const int *>(tensors[3]);
+  if (mp) p.from.table = static_cast<const int *>(tensors[4]);
+  p.k_out = tensors[5]; p.v_out = tensors[6];
+  if (mp_out) p.to.table = static_cast<const int *>(tensors[7]);
+  p.w_out = static_cast<float *>(tensors[8]);
+  p.seqlens_out = static_cast<int *>(tensors[9]);
+  p.kept = static_cast<int *>(tensors[10]);
+  if (!p.w || !p.seqlens || !p.w_out || !p.seqlens_out || !p.kept || (np > 0 && (!p.k || !p.v)) || (np_out > 0 && (!p.k_out || !p.v_out)) ||
+      (mp && !p.from.table) || (mp_out && !p.to.table))
+    return fail("null tensor pointer");
+  if (!aligned16(p.k) || !aligned16(p.v) || !aligned16(p.k_out) || !aligned16(p.v_out)) return fail("the caches must be 16-byte aligned");
+  // in place means the same rows under the same table; anything between that and two caches is refused
+  const bool k_same = p.k == p.k_out, v_same = p.v == p.v_out;
+  p.in_place = k_same && v_same;
+  const bool same_layout = st[0] == st[2] && st[1] == st[3] && st[4] == st[6] && st[5] == st[7] && st[8] == st[10] && st[9] == st[11] && np == np_out &&
+                           page == page_out && mp == mp_out && p.from.table == p.to.table;
+  if (k_same != v_same || (p.in_place && !same_layout)) return fail("in place, k_out, v_out and the output table must be the cache's own");
+  if (p.w == p.w_out && !p.in_place) return fail("weights can be moved in place only together with the caches");
+  return fa::launch_evict(p, static_cast<hipStream_t>(stream));
+}
+
 }  // namespace
 
 extern "C" {
+
+int flash_attn_sink_fwd_checked(void **tensors, const void *extra_args, int dtype, void *stream) {
+  return fwd_impl(tensors, extra_args, dtype, Scratch{nullptr, 0, nullptr}, stream, true);
+}
+int flash_attn_sink_bwd_checked(void **tensors, const void *extra_args, int dtype, void *stream) {
+  return bwd_impl(tensors, extra_args, dtype, Scratch{nullptr, 0, nullptr}, 0, stream, true);
+}
+int flash_attn_paged_checked(void **tensors, const void *extra_args, int dtype, void *stream) {
+  return paged_impl(tensors, extra_args, dtype, Scratch{nullptr, 0, nullptr}, stream);
+}
+int flash_attn_evict_checked(void **tensors, const void *extra_args, int dtype, void *stream) {
+  return evict_impl(tensors, extra_args, dtype, Scratch{nullptr, 0, nullptr}, stream);
+}
+int flash_attn_sink_fwd_ws(void **tensors, const void *extra_args, int dtype, void *workspace, size_t workspace_bytes, void *stream) {
+  return fwd_impl(tensors, extra_args, dtype, Scratch{workspace, workspace_bytes, nullptr}, stream, true);
+}
+int flash_attn_sink_bwd_ws(void **tensors, const void *extra_args, int dtype, void *workspace, size_t workspace_bytes, void *stream) {
+  return bwd_impl(tensors, extra_args, dtype, Scratch{workspace, workspace_bytes, nullptr}, 0, stream, true);
+}
+int flash_attn_paged_ws(void **tensors, const void *extra_args, int dtype, void *workspace, size_t workspace_bytes, void *stream) {
+  return paged_impl(tensors, extra_args, dtype, Scratch{workspace, workspace_bytes, nullptr}, stream);
+}
+int flash_attn_evict_ws(void **tensors, const void *extra_args, int dtype, void *workspace, size_t workspace_bytes, void *stream) {
+  return evict_impl(tensors, extra_args, dtype, Scratch{workspace, workspace_bytes, nullptr}, stream);
+}
+size_t flash_attn_sink_fwd_workspace_bytes(const void *extra_args, int dtype) {
+  size_t n = 0;
+  return fwd_impl(nullptr, extra_args, dtype, Scratch{nullptr, 0, &n}, nullptr, true) == 0 ? n : 0;
+}
+size_t flash_attn_sink_bwd_workspace_bytes(const void *extra_args, int dtype, size_t dq_accum_bytes) {
+  size_t n = 0;
+  return bwd_impl(nullptr, extra_args, dtype, Scratch{nullptr, 0, &n}, dq_accum_bytes, nullptr, true) == 0 ? n : 0;
+}
+size_t flash_attn_paged_workspace_bytes(const void *extra_args, int dtype) {
+  size_t n = 0;
+  return paged_impl(nullptr, extra_args, dtype, Scratch{nullptr, 0, &n}, nullptr) == 0 ? n : 0;
+}
+size_t flash_attn_evict_workspace_bytes(const void *extra_args, int dtype) {
+  size_t n = 0;
+  return evict_impl(nullptr, extra_args, dtype, Scratch{nullptr, 0, &n}, nullptr) == 0 ? n : 0;
+}
 
 int flash_attn_fwd_checked(void **tensors, const void *extra_args, int dtype, void *stream) {
   return fwd_impl(tensors, extra_args, dtype, Scratch{nullptr, 0, nullptr}, stream);
@@ -312,6 +516,30 @@ void run_flash_attn_kvcache_bf16(void **tensors, void *extra_args, void *stream)
 }
 void run_flash_attn_bwd_bf16(void **tensors, void *extra_args, void *stream) {
   if (int r = flash_attn_bwd_checked(tensors, extra_args, 2, stream)) die("run_flash_attn_bwd_bf16", r);
+}
+void run_flash_attn_sink_fwd(void **tensors, void *extra_args, void *stream) {
+  if (int r = flash_attn_sink_fwd_checked(tensors, extra_args, 1, stream)) die("run_flash_attn_sink_fwd", r);
+}
+void run_flash_attn_sink_fwd_bf16(void **tensors, void *extra_args, void *stream) {
+  if (int r = flash_attn_sink_fwd_checked(tensors, extra_args, 2, stream)) die("run_flash_attn_sink_fwd_bf16", r);
+}
+void run_flash_attn_sink_bwd(void **tensors, void *extra_args, void *stream) {
+  if (int r = flash_attn_sink_bwd_checked(tensors, extra_args, 1, stream)) die("run_flash_attn_sink_bwd", r);
+}
+void run_flash_attn_sink_bwd_bf16(void **tensors, void *extra_args, void *stream) {
+  if (int r = flash_attn_sink_bwd_checked(tensors, extra_args, 2, stream)) die("run_flash_attn_sink_bwd_bf16", r);
+}
+void run_flash_attn_paged(void **tensors, void *extra_args, void *stream) {
+  if (int r = flash_attn_paged_checked(tensors, extra_args, 1, stream)) die("run_flash_attn_paged", r);
+}
+void run_flash_attn_paged_bf16(void **tensors, void *extra_args, void *stream) {
+  if (int r = flash_attn_paged_checked(tensors, extra_args, 2, stream)) die("run_flash_attn_paged_bf16", r);
+}
+void run_flash_attn_evict(void **tensors, void *extra_args, void *stream) {
+  if (int r = flash_attn_evict_checked(tensors, extra_args, 1, stream)) die("run_flash_attn_evict", r);
+}
+void run_flash_attn_evict_bf16(void **tensors, void *extra_args, void *stream) {
+  if (int r = flash_attn_evict_checked(tensors, extra_args, 2, stream)) die("run_flash_attn_evict_bf16", r);
 }
 
 }  // extern "C"

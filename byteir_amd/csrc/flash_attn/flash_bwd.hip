@@ -88,6 +88,18 @@ struct TileLoader {
     }
   }
   __device__ __forceinline__ void gload() { gload_into(reg); }
+  // the tile that starts at row0, of which only the rows that are sinks or inside the block's
+  // window are read (the others arrive as zeros)
+  __device__ __forceinline__ void gload_seen(int64_t row_stride, int row0, const idx::SinkTiles &st) {
+    const int c = threadIdx.x % CPR, r = threadIdx.x / CPR;
+#pragma unroll
+    for (int s = 0; s < NP; ++s) {
+      const int row = row0 + r + s * RPP;
+      const bool seen = row < st.hi && (row >= st.lo || row < st.sink);
+      const u32x4 a = __builtin_amdgcn_raw_buffer_load_b128(rsrc, seen ? idx::chunk_offset(row, c, row_stride) : 0xffffffffu, 0, 0);
+      reg[s] = uint4{a.x, a.y, a.z, a.w};
+    }
+  }
   __device__ __forceinline__ void lstore_swz_from(T *tile, const uint4 (&rr)[NP]) const {
     const int c = threadIdx.x % CPR, r = threadIdx.x / CPR;
 #pragma unroll
@@ -169,7 +181,7 @@ __global__ void __launch_bounds__(256, (D <= 64 && KB == 1) ? 2 : 1) dkdv_kernel
     const T *vg = static_cast<const T *>(p.v) + bi * p.v_bs + (int64_t)kvcol[kb] * p.v_rs + hkv * p.v_hs;
 #pragma unroll
     for (int ks = 0; ks < D / 16; ++ks) {
-      if (kvcol[kb] < p.sk) {
+      if (kvcol[kb] < p.kv_hi && kvcol[kb] >= p.kv_lo) {
         kf[kb][ks] = *reinterpret_cast<const vec8 *>(kg + ks * 16 + g * 8);
         vf[kb][ks] = *reinterpret_cast<const vec8 *>(vg + ks * 16 + g * 8);
       } else {
@@ -512,7 +524,8 @@ __global__ void __launch_bounds__(256, (D <= 64 && KB == 1) ? 2 : 1) dkdv_kernel
 // under the exponentials, and the K / V fragments of a unit are fetched from LDS a step before
 // that.  Window edges are applied beforehand, by setting the masked scores
 // of an edge unit to -inf in a block of their own, which keeps B free of branches.
-template <typename T, int D>
+// Sink: as in flash_fwd.hip, the tiles of the sinks before those of the window.
+template <typename T, int D, bool Sink = false>
 __global__ void __launch_bounds__(256, D <= 64 ? 2 : 1) dq_kernel(const Params p) {
   using vec8 = typename Traits<T>::vec8;
   constexpr int KS = D;               // K tile: plain and transposed reads, laid out with Swz<D>
@@ -539,7 +552,14 @@ __global__ void __launch_bounds__(256, D <= 64 ? 2 : 1) dq_kernel(const Params p
   row_limits(p, wq0, w_lo_first, w_hi_first);
   row_limits(p, wq0 + 31, w_lo_last, w_hi_last);
   int n_min, n_max;
-  idx::key_tile_range(p.sq, p.sk, p.wl, p.wr, m0, kQBlock, kKvTile, n_min, n_max);
+  idx::SinkTiles st{};
+  if constexpr (Sink) {
+    st = idx::sink_tile_range(p.sq, p.sk, p.wl, p.wr, p.n_sink, m0, kQBlock, kKvTile);
+    n_min = 0;
+    n_max = st.n;
+  } else {
+    idx::key_tile_range(p.sq, p.sk, p.wl, p.wr, m0, kQBlock, kKvTile, n_min, n_max);
+  }
 
   const int hk = hi / (p.h / p.h_k);
   const T *kg = static_cast<const T *>(p.k) + bi * p.k_bs + hk * p.k_hs;
@@ -578,7 +598,17 @@ __global__ void __launch_bounds__(256, D <= 64 ? 2 : 1) dq_kernel(const Params p
   TileLoader<T, D, kKvTile> lk, lv;  // tiles are fetched in order, n_min first
   lk.start(kg, p.k_rs, n_min * kKvTile, p.sk);
   lv.start(vg, p.v_rs, n_min * kKvTile, p.sk);
-  auto gload = [&]() { lk.gload(); lv.gload(); };
+  int t_next = 0;  // Sink: the next tile to fetch
+  auto gload = [&]() {
+    if constexpr (Sink) {
+      const int kv0 = idx::sink_tile(st, t_next++) * kKvTile;
+      lk.gload_seen(p.k_rs, kv0, st);
+      lv.gload_seen(p.v_rs, kv0, st);
+    } else {
+      lk.gload();
+      lv.gload();
+    }
+  };
   auto lstore = [&](int buf) { lk.lstore_swz(Ks[buf]); lv.lstore(Vs[buf], VS); };
 
   struct Unit { float16v s, dp; };
@@ -589,8 +619,8 @@ __global__ void __launch_bounds__(256, D <= 64 ? 2 : 1) dq_kernel(const Params p
 
   // what the wave's 32 rows see of the 32 keys from kv0: 0 nothing, 1 all, 2 an edge crosses
   auto visibility = [&](int kv0) {
-    if (kv0 >= w_hi_last || kv0 + 32 <= w_lo_first) return 0;
-    return (kv0 + 32 > w_hi_first || kv0 < w_lo_last) ? 2 : 1;
+    if (kv0 >= w_hi_last || (kv0 + 32 <= w_lo_first && !(Sink && kv0 < p.n_sink))) return 0;
+    return (kv0 + 32 > w_hi_first || (kv0 < w_lo_last && !(Sink && kv0 + 32 <= p.n_sink))) ? 2 : 1;
   };
   // K and V fragments of one 32-key unit, fetched from LDS one step before the MFMAs that
   // use them, so that the LDS latency is not on the path of the step that consumes them
@@ -617,7 +647,7 @@ __global__ void __launch_bounds__(256, D <= 64 ? 2 : 1) dq_kernel(const Params p
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       const int kv = kv0 + (i >> 2) * 8 + g * 4 + (i & 3);
-      if (kv >= hi_lim || kv < lo_lim) u.s[i] = -INFINITY;
+      if (kv >= hi_lim || (kv < lo_lim && !(Sink && kv < p.n_sink))) u.s[i] = -INFINITY;
     }
   };
   // B: dS^T in place of S^T, packed as B operands [16-key window]
@@ -675,12 +705,13 @@ __global__ void __launch_bounds__(256, D <= 64 ? 2 : 1) dq_kernel(const Params p
   }
   // Under a right window (causal) the wave's rows see no key from w_hi_last on: it computes up
   // to the tile that holds that key and only keeps loading and meeting the barriers afterwards.
-  const int n_w_max = min(n_max, max(n_min, (w_hi_last + kKvTile - 1) / kKvTile));
+  const int n_w_end = (w_hi_last + kKvTile - 1) / kKvTile;
+  const int n_w_max = min(n_max, Sink ? st.ns + max(0, n_w_end - st.n0) : max(n_min, n_w_end));
   int buf = 0;  // ring slot of tile t
   for (int t = n_min; t < n_max; ++t) {
     const int buf1 = buf + 1 == kRing ? 0 : buf + 1;
     const int buf2 = buf1 + 1 == kRing ? 0 : buf1 + 1;
-    const int kv0 = t * kKvTile;
+    const int kv0 = (Sink ? idx::sink_tile(st, t) : t) * kKvTile;
     if (t > n_min) __syncthreads();  // tile t+1 is visible; every wave has left tile t-1
     // tile t+2: registers -> the ring slot tile t-1 occupied; tile t+3 in flight
     if (t + 2 < n_max) lstore(buf2);
@@ -783,7 +814,9 @@ hipError_t launch_bwd_td(const Params &p, hipStream_t stream) {
       return e != hipSuccess ? e : launch_dq_anyd128(p, std::is_same<T, _Float16>::value ? 1 : 2, stream);
     }
   }
-  if (pq.n_mblocks > 0)
+  if (pq.n_mblocks > 0 && p.sink)
+    FA_LAUNCH((dq_kernel<T, D, true>), dim3((unsigned)(pq.n_mblocks * p.b * p.h)), dim3(256), stream, pq);
+  else if (pq.n_mblocks > 0)
     FA_LAUNCH((dq_kernel<T, D>), dim3((unsigned)(pq.n_mblocks * p.b * p.h)), dim3(256), stream, pq);
   return hipGetLastError();
 }
@@ -814,11 +847,7 @@ hipError_t launch_group_sum(const Params &p, const GroupSplit &s, int row, int d
   return e;
 }
 
-hipError_t launch_bwd(Params &p, int dtype, hipStream_t stream) {
-  p.n_mblocks = (p.sq + kQBlock - 1) / kQBlock;
-  p.n_nblocks = (p.sk + kKvBlock - 1) / kKvBlock;
-  p.xcd_remap = idx::block_order_mode(p.b * p.h, p.wr);
-  if (p.b * p.h == 0) return hipSuccess;
+static hipError_t launch_bwd_all(Params &p, int dtype, hipStream_t stream) {
   // The tuned kernels address Q / dO / K / V tiles with 32-bit offsets inside a (batch, head)
   // slice (buffer loads), including a few tiles of look-ahead past the end: larger slices
   // take the generic kernels.
@@ -826,6 +855,29 @@ hipError_t launch_bwd(Params &p, int dtype, hipStream_t stream) {
   const int64_t span = idx::bwd_stream_span_bytes(std::max(p.sq, p.sk), max_rs);
   if (p.drop || (p.d != 32 && p.d != 64 && p.d != 128) || span >= (int64_t(1) << 31)) return launch_bwd_anyd(p, dtype, stream);
   return dtype == 1 ? launch_bwd_t<_Float16>(p, stream) : launch_bwd_t<__bf16>(p, stream);
+}
+
+hipError_t launch_bwd(Params &p, int dtype, hipStream_t stream) {
+  p.n_mblocks = (p.sq + kQBlock - 1) / kQBlock;
+  p.n_nblocks = (p.sk + kKvBlock - 1) / kKvBlock;
+  p.xcd_remap = idx::block_order_mode(p.b * p.h, p.wr);
+  p.kv_lo = 0;
+  p.kv_hi = p.sk;
+  if (p.b * p.h == 0) return hipSuccess;
+  if (!p.sink) return launch_bwd_all(p, dtype, stream);
+  // With sinks: dQ walks the sinks' tiles besides the window's, dK / dV come from the windowed
+  // kernel, and then the sinks' rows of dK / dV are replaced.  Scratch: the windowed call's, then the sinks'.
+  int hi;
+  idx::row_limits(p.sq, p.sk, p.wl, p.wr, 0, p.kv_lo, hi);
+  Params plan = p;
+  size_t base = 0;
+  plan.ws_query = &base;
+  if (hipError_t e = launch_bwd_all(plan, dtype, nullptr)) return e;
+  base = (base + 15) & ~(size_t)15;
+  if (p.ws_query) { *p.ws_query = base + sink_dkdv_bytes(p); return hipSuccess; }
+  if (hipError_t e = launch_bwd_all(p, dtype, stream)) return e;
+  const bool rest = p.ws && p.ws_bytes > base;
+  return launch_sink_dkdv(p, dtype, rest ? static_cast<char *>(p.ws) + base : nullptr, rest ? p.ws_bytes - base : 0, stream);
 }
 
 }  // namespace fa

@@ -189,6 +189,9 @@ struct Params {
   int sq, sk, sq_rounded;
   float scale, scale_log2;
   int wl, wr;                         // window sizes after normalisation; < 0 = unbounded
+  int sink;                           // 1: a flash_attn_sink_* call (the Sink kernels, also when n_sink is 0)
+  int n_sink;                         // the first n_sink keys stay visible outside the window
+  int kv_lo, kv_hi;                   // backward: the keys that some query row can see (dK/dV kernels load no others)
   int n_mblocks, n_nblocks;
   int xcd_remap;                      // 0: by (batch, head); 1: blocks of a (batch, head) share an XCD; 2: 1 + longest blocks of all heads first; 3: longest first without XCD grouping
   // key/value cache calls only: per-batch number of keys already in the cache (the cache
@@ -295,6 +298,11 @@ inline void apply_group_split(Params &pk, const Params &p, const GroupSplit &s, 
   pk.dk_bs = pk.dv_bs = (int64_t)p.sk * pk.h_k * row;
 }
 hipError_t launch_group_sum(const Params &p, const GroupSplit &s, int row, int dtype, hipStream_t stream);
+
+// dK / dV of the sink keys (flash_sink.hip): replaces the rows that the windowed kernel wrote;
+// sink_dkdv_bytes is the scratch it takes
+size_t sink_dkdv_bytes(const Params &p);
+hipError_t launch_sink_dkdv(const Params &p, int dtype, void *ws, size_t ws_bytes, hipStream_t stream);
 
 // A few query rows against a long key sequence (flash_decode.hip): all query heads of a
 // key/value head times all query rows must fit the 32 columns of one score tile.

@@ -36,7 +36,10 @@ constexpr float kRescaleSlack = 8.0f;
 
 // QB: 32-row halves per wave (1 or 2); NW: waves per workgroup; the workgroup owns 32*QB*NW rows
 // VarK: the number of keys is read per batch (key/value cache calls): seqlens_k[b] + seqlen_knew
-template <typename T, int D, int QB, int NW, bool VarK>
+// Sink: keys [0, p.n_sink) stay visible outside the window (idx::sink_tile_range): their tiles come
+// first, then the window's, as one list of tiles walked by the same loop; a tile row that none
+// of the workgroup's query rows can see is read as zeros, whatever it holds
+template <typename T, int D, int QB, int NW, bool VarK, bool Sink = false>
 __global__ void __launch_bounds__(NW * 64, NW * QB >= 16 ? 2 : (QB == 2 ? 1 : 2)) flash_fwd_kernel(const Params p) {
   constexpr int kThreads = NW * 64;
   constexpr int kBM = 32 * QB * NW;
@@ -78,8 +81,17 @@ __global__ void __launch_bounds__(NW * 64, NW * QB >= 16 ? 2 : (QB == 2 ? 1 : 2)
   }
   const int w_lo_first = h_lo_first[0], w_hi_last = h_hi_last[QB - 1];  // the wave's widest window
   // tile range of the workgroup
-  int n_min, n_max;
-  idx::key_tile_range(p.sq, sk, p.wl, p.wr, m0, kBM, kBN, n_min, n_max);
+  int n_min, n_max;  // Sink: positions in the list of tiles
+  idx::SinkTiles st{};
+  if constexpr (Sink) {
+    st = idx::sink_tile_range(p.sq, sk, p.wl, p.wr, p.n_sink, m0, kBM, kBN);
+    n_min = 0;
+    n_max = st.n;
+  } else {
+    idx::key_tile_range(p.sq, sk, p.wl, p.wr, m0, kBM, kBN, n_min, n_max);
+  }
+  // first key of the t-th tile
+  auto tile_kv0 = [&](int t) { return (Sink ? idx::sink_tile(st, t) : t) * kBN; };
   const int split = blockIdx.y;  // key axis split over workgroups: this one's share of the tiles
   if (p.n_splits > 1) {
     n_min = max(n_min, split * p.split_tiles);
@@ -130,7 +142,21 @@ __global__ void __launch_bounds__(NW * 64, NW * QB >= 16 ? 2 : (QB == 2 ? 1 : 2)
   }
   const unsigned k_tile_b = idx::tile_bytes(kBN, p.k_rs), v_tile_b = idx::tile_bytes(kBN, p.v_rs);
   unsigned k_so = (unsigned)n_min * k_tile_b, v_so = (unsigned)n_min * v_tile_b;  // byte offset of the next tile to fetch
+  int t_next = n_min;  // Sink: the next tile to fetch
   auto gload = [&]() {
+    if constexpr (Sink) {
+      const int kv0 = tile_kv0(t_next++);
+#pragma unroll
+      for (int s = 0; s < NP; ++s) {
+        const int row = kv0 + ld_r + s * RPP;
+        const bool seen = ld_on && row < st.hi && (row >= st.lo || row < st.sink);
+        const u32x4 a = __builtin_amdgcn_raw_buffer_load_b128(k_rsrc, seen ? idx::chunk_offset(row, ld_c, p.k_rs) : 0xffffffffu, 0, 0);
+        const u32x4 b = __builtin_amdgcn_raw_buffer_load_b128(v_rsrc, seen ? idx::chunk_offset(row, ld_c, p.v_rs) : 0xffffffffu, 0, 0);
+        kreg[s] = uint4{a.x, a.y, a.z, a.w};
+        vreg[s] = uint4{b.x, b.y, b.z, b.w};
+      }
+      return;
+    }
 #pragma unroll
     for (int s = 0; s < NP; ++s) {
       const u32x4 a = __builtin_amdgcn_raw_buffer_load_b128(k_rsrc, ld_on ? k_vo[s] + k_so : 0xffffffffu, 0, 0);
@@ -166,7 +192,7 @@ __global__ void __launch_bounds__(NW * 64, NW * QB >= 16 ? 2 : (QB == 2 ? 1 : 2)
   // pipelined inside each wave: the MFMAs of S^T for unit u+1 are independent of the softmax of
   // unit u, so they share a basic block and the exp/max/convert work runs in the MFMA shadow.
   // a wave sees nothing of a unit that lies wholly outside its widest row window
-  auto skipped = [&](int kv0) { return kv0 >= w_hi_last || kv0 + 32 <= w_lo_first; };
+  auto skipped = [&](int kv0) { return kv0 >= w_hi_last || (kv0 + 32 <= w_lo_first && !(Sink && kv0 < p.n_sink)); };
 
   struct Unit { float16v s[QB]; };  // S^T of one unit: [half]
 
@@ -186,11 +212,12 @@ __global__ void __launch_bounds__(NW * 64, NW * QB >= 16 ? 2 : (QB == 2 ? 1 : 2)
 #pragma unroll
     for (int qb = 0; qb < QB; ++qb) {
       float16v &sc = u.s[qb];
-      if (kv0 + 32 > h_hi_first[qb] || kv0 < h_lo_last[qb]) {  // a unit on the edge of the window
+      // a unit on the edge of the window
+      if (kv0 + 32 > h_hi_first[qb] || (kv0 < h_lo_last[qb] && !(Sink && kv0 + 32 <= p.n_sink))) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int kv = kv0 + (i >> 2) * 8 + g * 4 + (i & 3);
-          if (kv >= hi_lim[qb] || kv < lo_lim[qb]) sc[i] = -INFINITY;
+          if (kv >= hi_lim[qb] || (kv < lo_lim[qb] && !(Sink && kv < p.n_sink))) sc[i] = -INFINITY;
         }
       }
       float mx = -INFINITY;
@@ -220,8 +247,8 @@ __global__ void __launch_bounds__(NW * 64, NW * QB >= 16 ? 2 : (QB == 2 ? 1 : 2)
   // exponentials, row sums and P^T of one unit (branch free).  At head_dim 128 the row sum is
   // taken over the rounded P that the P V product uses, two elements per v_dot2c (fp32
   // accumulation), which halves the additions; at head_dim 64 that measured no faster and the
-  // sum stays on the unrounded exponentials.
-  constexpr bool kDotSum = D >= 128;
+  // sum stays on the unrounded exponentials; so it does with sinks, whose LSE is exact to fp32.
+  constexpr bool kDotSum = D >= 128 && !Sink;
   auto sm_exp = [&](Unit &u, vec8 (&pb)[QB][2]) {
 #pragma unroll
     for (int qb = 0; qb < QB; ++qb) {
@@ -303,13 +330,13 @@ __global__ void __launch_bounds__(NW * 64, NW * QB >= 16 ? 2 : (QB == 2 ? 1 : 2)
 #pragma unroll
     for (int s = 0; s < NP; ++s) { kreg[s] = k1[s]; vreg[s] = v1[s]; }
     __syncthreads();
-    if (!skipped(n_min * kBN)) qk(Ks[0], 0, ua);
+    if (!skipped(tile_kv0(n_min))) qk(Ks[0], 0, ua);
   }
   int buf = 0;  // ring slot of tile t
   for (int t = n_min; t < n_max; ++t) {
     const int buf1 = buf + 1 == kStages ? 0 : buf + 1;
     const int buf2 = buf1 + 1 == kStages ? 0 : buf1 + 1;
-    const int kv0 = t * kBN;
+    const int kv0 = tile_kv0(t), kv0_next = Sink ? tile_kv0(t + 1) : kv0 + kBN;
     // unit 0 of tile t (S in ua) while S of unit 1 is produced into ub
     step(!skipped(kv0), ua, kv0, Vs[buf], 0, !skipped(kv0 + 32), ub, Ks[buf], 1);
     __syncthreads();  // tile t+1 is visible; every wave has left tile t-1
@@ -317,7 +344,7 @@ __global__ void __launch_bounds__(NW * 64, NW * QB >= 16 ? 2 : (QB == 2 ? 1 : 2)
     if (t + 2 < n_max) lstore(buf2);
     if (t + 3 < n_max) gload();
     // unit 1 of tile t (S in ub) while S of unit 0 of tile t+1 is produced into ua
-    step(!skipped(kv0 + 32), ub, kv0 + 32, Vs[buf], 1, t + 1 < n_max && !skipped(kv0 + kBN), ua, Ks[buf1], 0);
+    step(!skipped(kv0 + 32), ub, kv0 + 32, Vs[buf], 1, t + 1 < n_max && !skipped(kv0_next), ua, Ks[buf1], 0);
     buf = buf1;
   }
 
@@ -440,7 +467,12 @@ hipError_t launch_fwd_d(Params &p, hipStream_t stream) {
   // num_splits_heuristic has the same aim, flash_api.cu:118-160, but its entry points never
   // enable it).  The partials live in the caller's workspace or, without one, in a
   // stream-ordered allocation; with neither: one split.
-  const int n_wg = p.n_mblocks * p.b * p.h, n_tiles = (p.sk + kBN - 1) / kBN;
+  const int n_wg = p.n_mblocks * p.b * p.h;
+  int n_tiles = (p.sk + kBN - 1) / kBN;
+  if (p.sink && p.wl >= 0 && p.wr >= 0) {  // with sinks the splits share out the list of tiles, which a window keeps short
+    const int64_t most = (int64_t)(std::min(p.n_sink, p.sk) + kBN - 1) / kBN + ((int64_t)p.wl + p.wr + BM) / kBN + 2;
+    n_tiles = (int)std::min<int64_t>(n_tiles, most);
+  }
   const int n_splits = pick_splits(n_wg, n_tiles);
   void *ws = nullptr;
   bool owned = false;
@@ -460,7 +492,8 @@ hipError_t launch_fwd_d(Params &p, hipStream_t stream) {
     p.ml_part = p.o_part + (size_t)n_splits * rows * D;
   }
   const dim3 grid((unsigned)n_wg, (unsigned)p.n_splits), block(NW * 64);
-  if (p.seqlens_k) FA_LAUNCH((flash_fwd_kernel<T, D, QB, NW, true>), grid, block, stream, p);
+  if (p.sink) FA_LAUNCH((flash_fwd_kernel<T, D, QB, NW, false, true>), grid, block, stream, p);
+  else if (p.seqlens_k) FA_LAUNCH((flash_fwd_kernel<T, D, QB, NW, true>), grid, block, stream, p);
   else FA_LAUNCH((flash_fwd_kernel<T, D, QB, NW, false>), grid, block, stream, p);
   hipError_t e = hipGetLastError();
   if (ws) {
@@ -519,7 +552,7 @@ hipError_t launch_append_kv(const Params &p, int dtype, hipStream_t stream) {
 hipError_t launch_fwd(Params &p, int dtype, hipStream_t stream) {
   p.xcd_remap = idx::block_order_mode(p.b * p.h, p.wr);
   if (p.b * p.h == 0 || p.sq == 0) return hipSuccess;
-  if (decode_eligible(p)) return launch_decode(p, dtype, stream);
+  if (!p.sink && decode_eligible(p)) return launch_decode(p, dtype, stream);
   // the tuned kernel addresses a head's K and V rows through 32-bit buffer offsets
   // (the padded rows of the last tile and the tiles of look-ahead that the prologue always
   // requests are part of the span: their offsets must not wrap either)

@@ -59,6 +59,28 @@ FA_HD void key_tile_range(int sq, int sk, int wl, int wr, int m0, int bm, int bn
   n_max = b_hi > 0 ? (b_hi + bn - 1) / bn : 0;
 }
 
+// A window with sinks: the first `n_sink` keys stay visible to every row that the right side of the
+// window lets see them.  Query rows [m0, m0 + bm) then visit `n` tiles: the first `ns` tiles of
+// the keys (those that hold sinks and lie before the window's first tile n0), then the window's;
+// the v-th of them is tile sink_tile(v).  [lo, hi) is the window of the block as a whole: keys
+// outside it that are no sinks are visible to none of its rows.
+struct SinkTiles { int ns, n0, n, lo, hi, sink; };
+FA_HD SinkTiles sink_tile_range(int sq, int sk, int wl, int wr, int n_sink, int m0, int bm, int bn) {
+  SinkTiles r;
+  int t0, t1, n1;
+  row_limits(sq, sk, wl, wr, m0, r.lo, t0);
+  const int last = m0 + bm < sq ? m0 + bm - 1 : sq - 1;
+  row_limits(sq, sk, wl, wr, last > m0 ? last : m0, t1, r.hi);
+  r.n0 = r.lo / bn;
+  n1 = r.hi > 0 ? (r.hi + bn - 1) / bn : 0;
+  r.sink = n_sink < r.hi ? n_sink : r.hi > 0 ? r.hi : 0;
+  const int s = (r.sink + bn - 1) / bn;
+  r.ns = s < r.n0 ? s : r.n0;
+  r.n = r.ns + (n1 > r.n0 ? n1 - r.n0 : 0);
+  return r;
+}
+FA_HD int sink_tile(const SinkTiles &r, int v) { return v < r.ns ? v : v - r.ns + r.n0; }
+
 // Query tiles [m_min, m_max) of `qt` rows that can see the keys [kv0, kv0 + keys); with
 // qsplit > 1 the share `q_share` of them.
 FA_HD void query_tile_range(int sq, int sk, int wl, int wr, int kv0, int keys, int qt, int qsplit, int q_share,

@@ -1,0 +1,402 @@
+// Attention of a few query rows (one new token, a draft, an observation window) over a key/value
+// cache in pages, with a window and sink keys, appending the new rows on the way
+// (flash_attn_paged):
+//   o_i = sum_j P_ij v_j,  P_ij = exp(scale q_i.k_j - lse_i),  j over the keys that row i sees,
+// and, when asked for, weights_j += sum of P_ij over the rows and the query heads that share
+// key/value head j belongs to.
+//
+// HBM-bound: every visible K and V row is read once.  The structure is that of flash_decode.hip:
+// the query heads of a key/value head times the query rows are the columns of one S^T tile (32
+// columns; more make more tiles), a wave streams units of 32 keys through registers into private
+// LDS tiles with the next unit in flight and no barrier in the loop, the waves join in LDS, the
+// workgroups that share a sequence's keys join through fp32 partials in a second kernel.
+// What differs: a unit's 32 row addresses come from the block table, looked up by one lane per row a
+// unit ahead of the loads that need them and handed round by lane permutes; the keys are cut by
+// the sequence's own length (units are numbered through sinks and window, and every sequence
+// shares its units out evenly over the splits the grid offers it), so a short sequence in a long
+// cache does not wait for one workgroup; rows that nobody sees (outside the window, behind the
+// last key, on an absent page) are not read and count as zeros.
+#include <algorithm>
+
+#include "flash_paged.h"
+
+namespace fa {
+namespace {
+
+constexpr int kWaves = 4;
+constexpr int kUnit = 32;  // keys per unit
+
+// D: the tile width, the smallest of 32, 64, 128, 256 that holds head_dim.  Scores: keep S for the weights.
+template <typename T, int D, bool Scores>
+__global__ void __launch_bounds__(kWaves * 64, D <= 128 ? 2 : 1) paged_kernel(const PagedParams p) {
+  using vec8 = typename Traits<T>::vec8;
+  constexpr int KS = Pad<D>::kPlain, VS = Pad<D>::kTr;
+  constexpr int CPR = D / 8;         // 16-byte chunks per row
+  constexpr int RPP = 64 / CPR;      // rows per pass of a wave
+  constexpr int NPV = kUnit / RPP;   // passes per unit
+  constexpr int kWaveLds = kUnit * (KS + VS) * (int)sizeof(T);  // a wave's K and V tile, reused for the join
+  static_assert(kWaveLds >= (D * 32 + 64) * 4, "join buffers must fit the tiles");
+  __shared__ __attribute__((aligned(16))) unsigned char lds[kWaves][kWaveLds];
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int r32 = lane & 31, g = lane >> 5;
+  const int split = blockIdx.x % p.n_splits;
+  const int ct = blockIdx.x / p.n_splits % p.n_ct;
+  const int bhk = blockIdx.x / p.n_splits / p.n_ct;
+  const int bi = bhk / p.h_k, hk = bhk % p.h_k;
+  const int group = p.h / p.h_k, n_cols = group * p.sq;
+  const int sk = p.keys_of(bi);
+
+  const idx::SinkTiles st = p.units(sk, ct);
+  const int n_units = min(st.n, p.max_units), per = p.per_split(n_units);
+  const int u0 = split * per, u1 = min(n_units, u0 + per);
+  if (split > 0 && u0 >= n_units) return;  // whole workgroups
+
+  // column n = ct * 32 + r32 of the S^T tile: query head hk*group + n / sq, query row n % sq
+  const int n = ct * 32 + r32;
+  const bool col_ok = n < n_cols;
+  const int qi = col_ok ? n % p.sq : 0, hq = hk * group + (col_ok ? n / p.sq : 0);
+  int lo_lim = 0, hi_lim = 0;
+  if (col_ok) idx::row_limits(p.sq, sk, p.wl, p.wr, qi, lo_lim, hi_lim);
+
+  const T *kg = static_cast<const T *>(p.k) + hk * p.pages.k_hs;
+  const T *vg = static_cast<const T *>(p.v) + hk * p.pages.v_hs;
+  vec8 qf[D / 16];
+  {
+    const T *qg = static_cast<const T *>(p.q) + bi * p.q_bs + (int64_t)qi * p.q_rs + hq * p.q_hs;
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks)
+      qf[ks] = (col_ok && ks * 16 + g * 8 < p.d) ? *reinterpret_cast<const vec8 *>(qg + ks * 16 + g * 8) : vec8{0};
+  }
+
+  T *Kt = reinterpret_cast<T *>(lds[wave]), *Vt = Kt + kUnit * KS;
+  uint4 kn[NPV], vn[NPV];
+  const int v_c = lane % CPR, v_r = lane / CPR;
+  typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+  // rows from new0 on come from k_new / v_new instead of the cache; the lane that loads one writes
+  // it to the cache (only where every new row is certain to be loaded: p.fuse_append)
+  const int new0 = p.fuse_append ? p.seqlens[bi] : 0x7fffffff;
+  const T *kng = p.fuse_append ? static_cast<const T *>(p.k_new) + bi * p.kn_bs + hk * p.kn_hs : nullptr;
+  const T *vng = p.fuse_append ? static_cast<const T *>(p.v_new) + bi * p.vn_bs + hk * p.vn_hs : nullptr;
+
+  // lane l holds the place of row l % 32 of the unit: its page (-1: nobody sees the row) and its row there
+  int pg_next = -1, row_next = 0, pg = -1;
+  auto locate = [&](int j) {
+    const int key = idx::sink_tile(st, j) * kUnit + r32;
+    pg_next = -1;
+    row_next = 0;
+    if (key < st.hi && (key >= st.lo || key < st.sink)) pg_next = p.pages.locate(bi, key, row_next);
+  };
+  auto load_unit = [&](int j) {  // unit j, whose rows locate(j) has found, into the staging registers
+    const int kv0 = idx::sink_tile(st, j) * kUnit;
+    const int pages = pg_next, rows = row_next;
+#pragma unroll
+    for (int s = 0; s < NPV; ++s) {
+      const int src = (s * RPP + v_r) * 4;
+      const int pgr = __builtin_amdgcn_ds_bpermute(src, pages), row = __builtin_amdgcn_ds_bpermute(src, rows);
+      if (pgr >= 0 && v_c * 8 < p.d) {  // columns from head_dim up to D stay zero
+        const int key = kv0 + s * RPP + v_r;
+        const bool fresh = key >= new0;
+        T *kc_row = const_cast<T *>(kg) + (int64_t)pgr * p.pages.k_ps + (int64_t)row * p.pages.k_rs + v_c * 8;
+        T *vc_row = const_cast<T *>(vg) + (int64_t)pgr * p.pages.v_ps + (int64_t)row * p.pages.v_rs + v_c * 8;
+        const T *ks_row = fresh ? kng + (int64_t)(key - new0) * p.kn_rs + v_c * 8 : kc_row;
+        const T *vs_row = fresh ? vng + (int64_t)(key - new0) * p.vn_rs + v_c * 8 : vc_row;
+        const u32x4 a = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(ks_row));
+        const u32x4 b = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(vs_row));
+        kn[s] = uint4{a.x, a.y, a.z, a.w};
+        vn[s] = uint4{b.x, b.y, b.z, b.w};
+        if (fresh) {
+          *reinterpret_cast<uint4 *>(kc_row) = kn[s];
+          *reinterpret_cast<uint4 *>(vc_row) = vn[s];
+        }
+      } else {  // zero rows: 0 * finite stays finite in P V
+        kn[s] = uint4{0, 0, 0, 0};
+        vn[s] = uint4{0, 0, 0, 0};
+      }
+    }
+  };
+  auto store_unit = [&]() {
+#pragma unroll
+    for (int s = 0; s < NPV; ++s) {
+      *reinterpret_cast<uint4 *>(&Kt[(s * RPP + v_r) * KS + v_c * 8]) = kn[s];
+      *reinterpret_cast<uint4 *>(&Vt[(s * RPP + v_r) * VS + v_c * 8]) = vn[s];
+    }
+    FA_WAVE_SYNC();  // the wave's own tile: written by all its lanes, read across lanes, no workgroup barrier
+  };
+
+  float16v o_acc[D / 32];
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) o_acc[i] = float16v{0};
+  float m_run = -INFINITY, l_run = 0.f;
+  const float c = p.scale_log2;
+
+  if (u0 + wave < u1) {
+    locate(u0 + wave);
+    load_unit(u0 + wave);
+    pg = pg_next;
+    if (u0 + wave + kWaves < u1) locate(u0 + wave + kWaves);
+    store_unit();
+  }
+  for (int j = u0 + wave; j < u1; j += kWaves) {
+    const bool has_next = j + kWaves < u1;
+    const uint32_t there = (uint32_t)__builtin_amdgcn_ballot_w64(pg >= 0);  // rows of unit j that were read
+    if (has_next) {
+      load_unit(j + kWaves);
+      pg = pg_next;
+      if (j + 2 * kWaves < u1) locate(j + 2 * kWaves);
+    }
+    float16v s = float16v{0};
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks)
+      s = Traits<T>::mfma(lds_read8<T>(&Kt[r32 * KS + ks * 16 + g * 8]), qf[ks], s);
+    const int kv0 = idx::sink_tile(st, j) * kUnit;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int r = (i >> 2) * 8 + g * 4 + (i & 3), kv = kv0 + r;
+      if (kv >= hi_lim || (kv < lo_lim && kv >= p.n_sink) || !((there >> r) & 1u)) s[i] = -INFINITY;
+    }
+    if constexpr (Scores) {
+      if (col_ok) {
+        float *sp = p.s_part + (((int64_t)bhk * n_cols + n) * p.max_units + j) * kUnit + g * 4;
+#pragma unroll
+        for (int i4 = 0; i4 < 4; ++i4)
+          *reinterpret_cast<float4 *>(sp + i4 * 8) = float4{s[i4 * 4], s[i4 * 4 + 1], s[i4 * 4 + 2], s[i4 * 4 + 3]};
+      }
+    }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[i]);
+    mx = fmaxf(mx, partner32(mx));
+    const float m_new = fmaxf(m_run, mx);
+    const float m_use = m_new == -INFINITY ? 0.f : m_new;
+    const float alpha = exp2_fast((m_run - m_use) * c);
+    const float m_scaled = m_use * c;
+    float rs = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float e = exp2_fast(fmaf(s[i], c, -m_scaled));
+      s[i] = e;
+      rs += e;
+    }
+    l_run = l_run * alpha + rs;
+    m_run = m_new;
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o_acc[db][i] *= alpha;
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      float pf[8];
+#pragma unroll
+      for (int jj = 0; jj < 8; ++jj) pf[jj] = s[w * 8 + jj];
+      const vec8 pb = pack8<T>(pf);  // P in the storage type: half a step of each term, as in the other kernels
+#pragma unroll
+      for (int db = 0; db < D / 32; ++db)
+        o_acc[db] = Traits<T>::mfma(lds_read_operand_tr<T>(Vt, VS, w * 16, db * 32), pb, o_acc[db]);
+    }
+    if (has_next) store_unit();  // after every read of unit j in program order
+  }
+
+  // ---- the four waves' partials joined through LDS (each wave writes into its own region) ----
+  const float l_wave = l_run + partner32(l_run);
+  float *Ow = reinterpret_cast<float *>(lds[wave]);  // [D][32]
+  float *MLw = Ow + D * 32;                          // [2][32]
+#pragma unroll
+  for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) Ow[(db * 32 + (i >> 2) * 8 + g * 4 + (i & 3)) * 32 + r32] = o_acc[db][i];
+  if (g == 0) { MLw[r32] = m_run; MLw[32 + r32] = l_wave; }
+  __syncthreads();
+
+  const int on = tid & 31, slice = tid >> 5;  // eight slices of D / 8 output elements per column
+  float mw[kWaves], wgt[kWaves], m_all = -INFINITY, l_all = 0.f;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    mw[w] = reinterpret_cast<const float *>(lds[w])[D * 32 + on];
+    m_all = fmaxf(m_all, mw[w]);
+  }
+  const float m_ref = m_all == -INFINITY ? 0.f : m_all;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    wgt[w] = exp2_fast((mw[w] - m_ref) * c);  // 0 for a wave that saw no key
+    l_all += wgt[w] * reinterpret_cast<const float *>(lds[w])[D * 32 + 32 + on];
+  }
+  const int cn = ct * 32 + on;
+  if (cn >= n_cols) return;
+  const int oi = cn % p.sq, oh = hk * group + cn / p.sq;
+  const bool final_pass = p.o_part == nullptr;
+  const bool empty = l_all == 0.f;
+  const float inv = final_pass ? (empty ? 1.f : 1.f / l_all) : 1.f;
+  T *og = static_cast<T *>(p.o) + bi * p.o_bs + (int64_t)oi * p.o_rs + oh * p.o_hs;
+  const int64_t prow = (((int64_t)split * p.b + bi) * p.h + oh) * p.sq + oi;
+#pragma unroll
+  for (int x = 0; x < D / 8; ++x) {
+    const int dcol = slice * (D / 8) + x;
+    float acc = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) acc += wgt[w] * reinterpret_cast<const float *>(lds[w])[dcol * 32 + on];
+    if (!final_pass) p.o_part[prow * D + dcol] = acc;
+    else if (dcol < p.d) og[dcol] = (T)(acc * inv);
+  }
+  if (slice == 0) {
+    if (final_pass) p.lse[((int64_t)bi * p.h + oh) * p.sq + oi] = empty ? INFINITY : m_all * p.scale + log2_fast(l_all) * kLn2;
+    else { p.ml_part[prow * 2] = m_all; p.ml_part[prow * 2 + 1] = l_all; }
+  }
+}
+
+// joins the splits' partials of one (sequence, head, query row) per workgroup, one thread per output
+// element; n_splits <= 64, so lane s of every wave takes split s for the statistics
+template <typename T, int D>
+__global__ void __launch_bounds__(D < 64 ? 64 : D) paged_join_kernel(const PagedParams p) {
+  __shared__ float wgt[64];
+  const int64_t row = blockIdx.x, rows = (int64_t)p.b * p.h * p.sq;  // (sequence * h + head) * sq + query row
+  const int qi = (int)(row % p.sq), hq = (int)(row / p.sq % p.h), bi = (int)(row / p.sq / p.h);
+  const int n_units = min(p.units(p.keys_of(bi), (hq % (p.h / p.h_k) * p.sq + qi) / 32).n, p.max_units);
+  const int per = p.per_split(n_units), n_live = max(1, (n_units + per - 1) / per);
+  const int dcol = threadIdx.x < D ? threadIdx.x : D - 1, lane = threadIdx.x & 63;  // whole waves only
+  const bool has = lane < n_live;
+  const float m_s = has ? p.ml_part[(lane * rows + row) * 2] : -INFINITY;
+  const float l_s = has ? p.ml_part[(lane * rows + row) * 2 + 1] : 0.f;
+  float m_all = m_s;
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) m_all = fmaxf(m_all, __shfl_xor(m_all, off, 64));
+  const float m_ref = m_all == -INFINITY ? 0.f : m_all;
+  const float w_s = exp2_fast((m_s - m_ref) * p.scale_log2);  // 0 for a split that saw no key
+  float l_all = w_s * l_s;
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) l_all += __shfl_xor(l_all, off, 64);
+  if (threadIdx.x < 64) wgt[threadIdx.x] = w_s;
+  __syncthreads();
+  float acc = 0.f;
+  const float *op = p.o_part + row * D + dcol;
+#pragma unroll 8
+  for (int s = 0; s < n_live; ++s) acc += wgt[s] * op[s * rows * D];
+  const bool empty = l_all == 0.f;
+  T *og = static_cast<T *>(p.o) + bi * p.o_bs + (int64_t)qi * p.o_rs + hq * p.o_hs;
+  if (threadIdx.x < p.d) og[dcol] = (T)(empty ? 0.f : acc / l_all);
+  if (threadIdx.x == 0) p.lse[row] = empty ? INFINITY : m_all * p.scale + log2_fast(l_all) * kLn2;
+}
+
+// weights_out[key] = weights_in[key] (0 for a row appended by this call) + sum of P over the columns of
+// the key/value head, in column order; a thread per key, keys behind the last one are left alone
+__global__ void __launch_bounds__(256) paged_weights_kernel(const PagedParams p) {
+  const int blocks = (p.pages.capacity() + 255) / 256;
+  const int bhk = blockIdx.x / blocks, bi = bhk / p.h_k, hk = bhk % p.h_k;
+  const int key = blockIdx.x % blocks * 256 + threadIdx.x, sk = p.keys_of(bi);
+  if (key >= sk) return;
+  const int group = p.h / p.h_k, n_cols = group * p.sq;
+  const int64_t at = (int64_t)bhk * p.pages.capacity() + key;
+  float w = p.w_in && key < p.seqlens[bi] ? p.w_in[at] : 0.f;
+  const int tile = key / kUnit;
+  for (int ct = 0; ct < p.n_ct; ++ct) {
+    const idx::SinkTiles st = p.units(sk, ct);
+    const int j = tile < st.ns ? tile : tile - st.n0 + st.ns;  // the unit that holds the key
+    if ((tile >= st.ns && tile < st.n0) || j >= min(st.n, p.max_units)) continue;
+    const int c1 = min(n_cols, (ct + 1) * 32);
+    for (int n = ct * 32; n < c1; ++n) {
+      const float s = p.s_part[(((int64_t)bhk * n_cols + n) * p.max_units + j) * kUnit + key % kUnit];
+      const float lse = p.lse[((int64_t)bi * p.h + hk * group + n / p.sq) * p.sq + n % p.sq];
+      w += s == -INFINITY ? 0.f : exp2_fast(fmaf(s, p.scale_log2, -lse * kLog2e));
+    }
+  }
+  p.w_out[at] = w;
+}
+
+// the new rows into the cache, 16 bytes a thread; rows behind the capacity or on an absent page are dropped
+__global__ void __launch_bounds__(256) paged_append_kernel(const PagedParams p) {
+  const int cpr = p.d / 8;
+  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (e >= (int64_t)p.b * p.n_new * p.h_k * cpr) return;
+  const int c = (int)(e % cpr), hk = (int)(e / cpr % p.h_k);
+  const int i = (int)(e / cpr / p.h_k % p.n_new), bi = (int)(e / cpr / p.h_k / p.n_new);
+  const int old = p.seqlens[bi];
+  if (old < 0 || (int64_t)old + i >= p.pages.capacity()) return;
+  int row;
+  const int pg = p.pages.locate(bi, old + i, row);
+  if (pg < 0) return;
+  typedef unsigned short u16;  // either storage type
+  const u16 *ks = static_cast<const u16 *>(p.k_new) + bi * p.kn_bs + (int64_t)i * p.kn_rs + hk * p.kn_hs + c * 8;
+  const u16 *vs = static_cast<const u16 *>(p.v_new) + bi * p.vn_bs + (int64_t)i * p.vn_rs + hk * p.vn_hs + c * 8;
+  u16 *kd = static_cast<u16 *>(const_cast<void *>(p.k)) + (int64_t)pg * p.pages.k_ps + (int64_t)row * p.pages.k_rs + hk * p.pages.k_hs + c * 8;
+  u16 *vd = static_cast<u16 *>(const_cast<void *>(p.v)) + (int64_t)pg * p.pages.v_ps + (int64_t)row * p.pages.v_rs + hk * p.pages.v_hs + c * 8;
+  *reinterpret_cast<uint4 *>(kd) = *reinterpret_cast<const uint4 *>(ks);
+  *reinterpret_cast<uint4 *>(vd) = *reinterpret_cast<const uint4 *>(vs);
+}
+
+template <typename T, int D>
+hipError_t paged_td(PagedParams &p, hipStream_t stream) {
+  const int64_t rows = (int64_t)p.b * p.h * p.sq;
+  const size_t s_bytes = p.w_out ? (size_t)p.b * p.h_k * (p.h / p.h_k) * p.sq * p.max_units * kUnit * sizeof(float) : 0;
+  const size_t o_bytes = p.n_splits > 1 ? (size_t)p.n_splits * rows * (D + 2) * sizeof(float) : 0;
+  const size_t need = s_bytes + o_bytes;
+  if (p.ws_query) { *p.ws_query = need; return hipSuccess; }
+  void *ws = nullptr;
+  bool owned = false;
+  if (need) {
+    if (p.ws && (reinterpret_cast<uintptr_t>(p.ws) & 15) == 0 && p.ws_bytes >= need) ws = p.ws;
+    else if (hipMallocAsync(&ws, need, stream) == hipSuccess) owned = true;
+    else { (void)hipGetLastError(); ws = nullptr; }
+    if (!ws && s_bytes) return hipErrorOutOfMemory;  // the scores have nowhere to go
+    if (!ws) p.n_splits = 1;
+    else {
+      p.s_part = s_bytes ? static_cast<float *>(ws) : nullptr;
+      if (o_bytes) {
+        p.o_part = static_cast<float *>(ws) + s_bytes / sizeof(float);
+        p.ml_part = p.o_part + (size_t)p.n_splits * rows * D;
+      }
+    }
+  }
+  hipError_t e = hipSuccess;
+  if (p.n_new > 0 && !p.fuse_append) {
+    const int64_t n = (int64_t)p.b * p.n_new * p.h_k * (p.d / 8);
+    FA_LAUNCH((paged_append_kernel), dim3((unsigned)((n + 255) / 256)), dim3(256), stream, p);
+    e = hipGetLastError();
+  }
+  const dim3 grid((unsigned)((int64_t)p.b * p.h_k * p.n_ct * p.n_splits));
+  if (e == hipSuccess) {
+    if (p.w_out) FA_LAUNCH((paged_kernel<T, D, true>), grid, dim3(kWaves * 64), stream, p);
+    else FA_LAUNCH((paged_kernel<T, D, false>), grid, dim3(kWaves * 64), stream, p);
+    e = hipGetLastError();
+  }
+  if (e == hipSuccess && p.o_part) {
+    FA_LAUNCH((paged_join_kernel<T, D>), dim3((unsigned)rows), dim3(D < 64 ? 64 : D), stream, p);
+    e = hipGetLastError();
+  }
+  if (e == hipSuccess && p.w_out) {
+    FA_LAUNCH((paged_weights_kernel), dim3((unsigned)((int64_t)((p.pages.capacity() + 255) / 256) * p.b * p.h_k)), dim3(256), stream, p);
+    e = hipGetLastError();
+  }
+  if (owned) {
+    const hipError_t f = hipFreeAsync(ws, stream);
+    if (e == hipSuccess) e = f;
+  }
+  return e;
+}
+
+template <typename T>
+hipError_t paged_t(PagedParams &p, hipStream_t stream) {
+  if (p.d <= 32) return paged_td<T, 32>(p, stream);
+  if (p.d <= 64) return paged_td<T, 64>(p, stream);
+  if (p.d <= 128) return paged_td<T, 128>(p, stream);
+  return paged_td<T, 256>(p, stream);
+}
+
+}  // namespace
+
+hipError_t launch_paged(PagedParams &p, int dtype, hipStream_t stream) {
+  const int cap = p.pages.capacity();
+  p.n_ct = (p.h / p.h_k * p.sq + 31) / 32;
+  // most units a tile visits: the sinks' and those of a window over its rows, or the whole cache
+  int64_t units = (cap + kUnit - 1) / kUnit;
+  if (p.wl >= 0)
+    units = std::min<int64_t>(units, (std::min(p.n_sink, cap) + kUnit - 1) / kUnit + ((int64_t)p.wl + p.sq + kUnit) / kUnit + 2);
+  p.max_units = (int)std::max<int64_t>(units, 1);
+  const int64_t base = (int64_t)p.b * p.h_k * p.n_ct;
+  p.min_units = kWaves;
+  p.n_splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>((1024 + base - 1) / base, 64), p.max_units / (2 * kWaves)));
+  // the attention kernel appends when one workgroup's tile covers all columns and its window reaches the first new row
+  p.fuse_append = p.n_new > 0 && p.n_ct == 1 && (p.wl < 0 || p.n_new <= (int64_t)p.sq + p.wl);
+  return dtype == 1 ? paged_t<_Float16>(p, stream) : paged_t<__bf16>(p, stream);
+}
+
+}  // namespace fa

@@ -178,8 +178,8 @@ def flash_attn_workspace_bytes(kind, dtype, blob, dq_accum_bytes=0):
     L = _lib.flash_attn()
     buf = ctypes.create_string_buffer(blob, len(blob))
     code = 1 if dtype == torch.float16 else 2
-    if kind == "bwd":
-        return L.flash_attn_bwd_workspace_bytes(ctypes.cast(buf, ctypes.c_void_p), code, dq_accum_bytes)
+    if kind in ("bwd", "sink_bwd"):
+        return getattr(L, f"flash_attn_{kind}_workspace_bytes")(ctypes.cast(buf, ctypes.c_void_p), code, dq_accum_bytes)
     return getattr(L, f"flash_attn_{kind}_workspace_bytes")(ctypes.cast(buf, ctypes.c_void_p), code)
 
 
@@ -276,3 +276,266 @@ def flash_attn_kvcache(q, kcache, vcache, knew, vnew, seqlens_k, scale, window=(
     fn = L.run_flash_attn_kvcache if q.dtype == torch.float16 else L.run_flash_attn_kvcache_bf16
     _call_custom(fn, [q, kcache, vcache, knew, vnew, seqlens_k, o, lse], blob, stream)
     return o, lse
+
+
+# ---- attention with a window and sinks, over a paged cache, and eviction from a cache -----------
+def _on(device, *tensors):
+    """Every tensor given lies on `device` (a GPU)."""
+    if device.type != "cuda":
+        raise ValueError("device tensor required: the ROCm provider has no host path")
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise ValueError(f"tensors on {device} and {t.device}: one call takes tensors of one GPU")
+
+
+def _like(t, dtype, shape, what):
+    if t is not None and (t.dtype != dtype or tuple(t.shape) != tuple(shape)):
+        raise ValueError(f"{what} must be {dtype} {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
+
+
+def _dense(t, what):
+    if t is not None and not t.is_contiguous():
+        raise ValueError(f"{what} must be dense row-major")
+
+
+def _half(q, *tensors):
+    if q.dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError(f"{q.dtype} is not supported (float16 or bfloat16)")
+    for t in tensors:
+        if t is not None and t.dtype != q.dtype:
+            raise ValueError(f"tensors of {q.dtype} and {t.dtype}: one call takes one storage type")
+    for t in (q,) + tensors:
+        if t is not None and (t.dim() != 4 or (t.numel() and t.stride(3) != 1)):
+            raise ValueError("4-d tensors with a dense head_dim required")
+
+
+def _strides(t):
+    """(outer, row, head) strides; an axis of length 1 has none that counts."""
+    return [t.stride(i) if t.shape[i] > 1 else 0 for i in range(3)] if t is not None else [0, 0, 0]
+
+
+def _overlaps(t):
+    """Whether elements of a view may share memory (an expanded axis, say)."""
+    end = 0
+    for stride, n in sorted((t.stride(i), t.shape[i]) for i in range(t.dim()) if t.shape[i] > 1):
+        if stride <= end:
+            return True
+        end += stride * (n - 1)
+    return False
+
+
+def _call_checked(kind, tensors, blob, device, dtype, workspace, stream, dq_accum_bytes=0):
+    """flash_attn_<kind>_ws on the tensors' own GPU, with the caller's scratch or scratch from torch's
+    allocator; raises ValueError for a call that the library refuses."""
+    with torch.cuda.device(device):
+        stream = stream if stream is not None else torch.cuda.current_stream()
+        if workspace is None:
+            need = flash_attn_workspace_bytes(kind, dtype, blob, dq_accum_bytes)
+            if need:
+                workspace = torch.empty(need, dtype=torch.uint8, device=device)
+                workspace.record_stream(stream)
+        _call_custom_ws(kind, dtype, tensors, blob, workspace, stream)
+
+
+def _check_sink(q, k, v, o):
+    _half(q, k, v, o)
+    b, sq, h, d = q.shape
+    if k.shape != v.shape or k.shape[0] != b or k.shape[3] != d:
+        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not fit together")
+
+
+def pack_flash_sink_args(q, k, v, o, scale, window, n_sink):
+    """The 200-byte extra_args blob of flash_attn_sink_fwd / _bwd: pack_flash_args, then i64 n_sink."""
+    return pack_flash_args(q, k, v, o, scale, window) + struct.pack("<q", n_sink)
+
+
+def flash_attn_sink_fwd(q, k, v, scale, window=(-1, 0), n_sink=0, stream=None, out=None, workspace=None):
+    """Attention in which row i sees the keys of its window, as in flash_attn_fwd, and of the first
+    `n_sink` keys those that the window's right side admits: q [b, sq, h, d], k, v [b, sk, h_k, d]
+    -> (o [b, sq, h, d], lse [b, h, sq] f32).  lse comes from unrounded fp32 sums at every
+    head_dim.  A row that sees no key gives o = 0, lse = +inf.  A key that no row of a 256-row
+    block sees may hold anything; a NaN in a key that some row sees may reach the rows beside it.
+    out: optional (o, lse) to write into; workspace: optional uint8 device tensor of
+    flash_attn_workspace_bytes("sink_fwd", ...) bytes."""
+    _check_sink(q, k, v, None)
+    b, sq, h, d = q.shape
+    o, lse = out if out is not None else (torch.empty((b, sq, h, d), dtype=q.dtype, device=q.device),
+                                          torch.empty((b, h, sq), dtype=torch.float32, device=q.device))
+    _half(q, o)
+    _like(o, q.dtype, q.shape, "o")
+    _like(lse, torch.float32, (b, h, sq), "lse")
+    _dense(lse, "lse")
+    _on(q.device, k, v, o, lse, workspace)
+    _call_checked("sink_fwd", [q, k, v, None, o, lse, None], pack_flash_sink_args(q, k, v, o, scale, window, n_sink), q.device, q.dtype, workspace, stream)
+    return o, lse
+
+
+def flash_attn_sink_bwd(dout, q, k, v, o, lse, scale, window=(-1, 0), n_sink=0, stream=None, out=None, workspace=None):
+    """Gradients of flash_attn_sink_fwd -> (dq, dk, dv), laid out as q, k, v (densely where one is a
+    broadcast view); dk and dv of a
+    key/value head are the sums over its query heads.  o and lse are the forward call's.
+    out: optional (dq, dk, dv, d_softmax, dq_accum, _) of flash_attn_bwd_buffers."""
+    _check_sink(q, k, v, o)
+    _half(q, dout)
+    b, sq, h, d = q.shape
+    _like(o, q.dtype, q.shape, "o")
+    _like(dout, q.dtype, q.shape, "dout")
+    _like(lse, torch.float32, (b, h, sq), "lse")
+    _dense(lse, "lse")
+    if _strides(dout) != _strides(o):  # the library addresses dout with the strides of o
+        dout = torch.empty_strided(o.shape, o.stride(), dtype=o.dtype, device=o.device).copy_(dout)
+    # gradients are written with the strides of q, k, v: a broadcast one is laid out densely first
+    q, k, v = (t.contiguous() if _overlaps(t) else t for t in (q, k, v))
+    if out is None:
+        like = lambda t: torch.empty_strided(t.shape, t.stride(), dtype=t.dtype, device=t.device)
+        # the grouped heads' partials go into the workspace, not into a dq_accum tensor
+        out = (like(q), like(k), like(v), torch.empty((b, h, round_up(sq, 128)), dtype=torch.float32, device=q.device), None, None)
+    dq, dk, dv, dsm, dq_accum, _ = out
+    for g, t, what in ((dq, q, "dq"), (dk, k, "dk"), (dv, v, "dv")):
+        _like(g, t.dtype, t.shape, what)
+        if _strides(g) != _strides(t):
+            raise ValueError(f"{what} must be laid out as {what[1:]}")
+    _like(dsm, torch.float32, (b, h, round_up(sq, 128)), "d_softmax")
+    _dense(dsm, "d_softmax")
+    if dq_accum is not None:
+        _like(dq_accum, torch.float32, (b, round_up(sq, 128), h, round_up(d, 32)), "dq_accum")
+        _dense(dq_accum, "dq_accum")
+    _on(q.device, dout, k, v, o, lse, dq, dk, dv, dsm, dq_accum, workspace)
+    _call_checked("sink_bwd", [dout, q, k, v, o, lse, None, dq, dk, dv, dsm, dq_accum], pack_flash_sink_args(q, k, v, o, scale, window, n_sink),
+                  q.device, q.dtype, workspace, stream, dq_accum.numel() * 4 if dq_accum is not None else 0)
+    return dq, dk, dv
+
+
+def pack_flash_paged_args(q, k_pages, v_pages, k_new, v_new, o, scale, window, n_sink, max_pages, weights):
+    """The 252-byte extra_args blob of flash_attn_paged: 18 strides in the order of the kvcache blob (the
+    caches' outer stride is that of a page), i64 b, h, h_k, d, seqlen_knew; f32 scale; i64 seqlen_q,
+    num_pages, page_size, max_pages, window left, right, n_sink, weights (0 none, 1 from zero, 2 on top
+    of weights)."""
+    b, sq, h, d = q.shape
+    each = [_strides(t) for t in (q, k_pages, v_pages, k_new, v_new, o)]
+    ints1 = [s[i] for i in range(3) for s in each] + [b, h, k_pages.shape[2], d, k_new.shape[1] if k_new is not None else 0]
+    ints2 = [sq, k_pages.shape[0], k_pages.shape[1], max_pages, window[0], window[1], n_sink, weights]
+    return struct.pack("<23q", *ints1) + struct.pack("<f", scale) + struct.pack("<8q", *ints2)
+
+
+def flash_attn_paged(q, k_pages, v_pages, block_table, seqlens_k, scale, window=(-1, 0), n_sink=0, k_new=None, v_new=None, weights=None,
+                     weights_out=None, stream=None, out=None, workspace=None):
+    """Attention of a few query rows over a key/value cache in pages.  q [b, sq, h, d]; k_pages, v_pages
+    [num_pages, page_size, h_k, d]; block_table int32 [b, max_pages]: row j of sequence i is row
+    j % page_size of page block_table[i][j // page_size].  block_table None: a dense cache
+    [b, capacity, h_k, d].  seqlens_k int32 [b]: rows in the cache before the call; a negative length
+    marks an idle sequence (o = 0, lse = +inf, nothing appended).
+    k_new, v_new [b, n, h_k, d] are written to the cache IN PLACE at rows seqlens_k[i].. first; rows
+    behind the capacity are dropped.  q then attends to rows [0, seqlens_k[i] + n) with the window
+    aligned to their end, plus the first n_sink rows (see flash_attn_sink_fwd).  Keys on a page whose
+    number lies outside the pool are not seen; rows that no query row sees are not read.  A page
+    that receives new rows must appear once, in one sequence's table.
+    weights / weights_out f32 [b, h_k, capacity] (weights_out may be weights): when weights_out is given,
+    weights_out[i, c, j] = weights[i, c, j] (0 without weights, and for rows appended by this call) + the
+    attention that key j got from all query rows and heads of key/value head c, for the rows j in
+    the cache after the call; the others are left as they were.
+    -> (o, lse[b, h, sq] f32), and weights_out when given."""
+    _half(q, k_pages, v_pages, k_new, v_new)
+    b, sq, h, d = q.shape
+    hk = k_pages.shape[2]
+    if k_pages.shape != v_pages.shape or k_pages.shape[3] != d:
+        raise ValueError(f"q {tuple(q.shape)}, k_pages {tuple(k_pages.shape)} and v_pages {tuple(v_pages.shape)} do not fit together")
+    if (k_new is None) != (v_new is None):
+        raise ValueError("k_new and v_new must be given together")
+    if k_new is not None:
+        if _overlaps(k_pages) or _overlaps(v_pages):
+            raise ValueError("new rows cannot be written to a broadcast view")
+        for t in (k_new, v_new):
+            _like(t, q.dtype, (b, k_new.shape[1], hk, d), "k_new / v_new")
+    if weights is not None and weights_out is None:
+        raise ValueError("weights without weights_out")
+    max_pages = 0
+    if block_table is not None:
+        if block_table.dim() != 2 or block_table.shape[1] == 0:
+            raise ValueError("block_table must be [b, max_pages] with at least one page")
+        _like(block_table, torch.int32, (b, block_table.shape[1]), "block_table")
+        max_pages = block_table.shape[1]
+    elif k_pages.shape[0] != b:
+        raise ValueError(f"{b} sequences, but a dense cache of {k_pages.shape[0]}")
+    cap = (max_pages or 1) * k_pages.shape[1]
+    _like(seqlens_k, torch.int32, (b,), "seqlens_k")
+    o, lse = out if out is not None else (torch.empty((b, sq, h, d), dtype=q.dtype, device=q.device),
+                                          torch.empty((b, h, sq), dtype=torch.float32, device=q.device))
+    _half(q, o)
+    _like(o, q.dtype, q.shape, "o")
+    _like(lse, torch.float32, (b, h, sq), "lse")
+    for t, what in ((weights, "weights"), (weights_out, "weights_out")):
+        _like(t, torch.float32, (b, hk, cap), what)
+        _dense(t, what)
+    for t, what in ((lse, "lse"), (block_table, "block_table"), (seqlens_k, "seqlens_k")):
+        _dense(t, what)
+    _on(q.device, k_pages, v_pages, k_new, v_new, block_table, seqlens_k, o, lse, weights, weights_out, workspace)
+    mode = 0 if weights_out is None else 1 if weights is None else 2
+    blob = pack_flash_paged_args(q, k_pages, v_pages, k_new, v_new, o, scale, window, n_sink, max_pages, mode)
+    _call_checked("paged", [q, k_pages, v_pages, k_new, v_new, block_table, seqlens_k, o, lse, weights, weights_out], blob, q.device, q.dtype, workspace, stream)
+    return (o, lse) if weights_out is None else (o, lse, weights_out)
+
+
+def pack_flash_evict_args(k, v, k_out, v_out, b, max_pages, max_pages_out, budget, n_sink, n_recent):
+    """The 192-byte extra_args blob of flash_attn_evict, 24 i64: the outer (page), row and head strides of k, v,
+    k_out, v_out; b, h_k, d; num_pages, page_size, max_pages of the cache and of the output cache; budget,
+    n_sink, n_recent."""
+    each = [_strides(t) for t in (k, v, k_out, v_out)]
+    return struct.pack("<24q", *[s[i] for i in range(3) for s in each], b, k.shape[2], k.shape[3], k.shape[0], k.shape[1], max_pages,
+                       k_out.shape[0], k_out.shape[1], max_pages_out, budget, n_sink, n_recent)
+
+
+def flash_attn_evict(k, v, weights, seqlens_k, budget, n_sink=0, n_recent=0, block_table=None, k_out=None, v_out=None, out_table=None,
+                     weights_out=None, seqlens_out=None, kept=None, stream=None):
+    """Cuts every (sequence, key/value head) of a cache to `budget` rows: the first n_sink, the last n_recent
+    and, of those between, the ones of greatest weight (equal weights: the lower row; NaN below everything)
+    stay and move to the front in their order.  k, v: pages with block_table, or dense [b, s, h_k, d];
+    weights f32 [b, h_k, capacity] (what flash_attn_paged accumulates); seqlens_k int32 [b].
+    Without k_out / v_out the cache, weights and seqlens_k are updated IN PLACE; with them (pages with
+    out_table, or dense) the rows that stay are copied there and the cache is left alone.  A sequence of
+    at most `budget` rows keeps them all; a negative length stays.  Rows, weights behind the last kept
+    one and rows of absent pages are left as they were.
+    -> (kept int32 [b, h_k, budget]: the row each came from, -1 behind the last; weights_out; seqlens_out)."""
+    _half(k, v, k_out, v_out)
+    if k.shape != v.shape:
+        raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} do not fit together")
+    if (k_out is None) != (v_out is None):
+        raise ValueError("k_out and v_out must be given together")
+    b, hk = seqlens_k.shape[0] if seqlens_k.dim() == 1 else -1, k.shape[2]
+    in_place = k_out is None
+    if in_place:
+        if out_table is not None:
+            raise ValueError("out_table without k_out")
+        k_out, v_out, out_table = k, v, block_table
+    elif k_out.shape != v_out.shape or k_out.shape[2:] != k.shape[2:]:
+        raise ValueError(f"k_out {tuple(k_out.shape)} and v_out {tuple(v_out.shape)} do not fit k {tuple(k.shape)}")
+    if _overlaps(k_out) or _overlaps(v_out):
+        raise ValueError("rows cannot be moved to a broadcast view")
+    caps = []
+    for t, pages, what in ((block_table, k, "block_table"), (out_table, k_out, "out_table")):
+        if t is not None and (t.dim() != 2 or t.shape[1] == 0):
+            raise ValueError(f"{what} must be [b, max_pages] with at least one page")
+        if t is None and pages.shape[0] != b:
+            raise ValueError(f"{b} sequences, but a dense cache of {pages.shape[0]}")
+        if t is not None:
+            _like(t, torch.int32, (b, t.shape[1]), what)
+        _dense(t, what)
+        caps.append((t.shape[1] if t is not None else 1) * pages.shape[1])
+    if weights_out is None:
+        weights_out = weights if in_place else torch.zeros((b, hk, caps[1]), dtype=torch.float32, device=k.device)
+    if seqlens_out is None:
+        seqlens_out = seqlens_k if in_place else torch.empty_like(seqlens_k)
+    if kept is None:
+        kept = torch.empty((b, hk, max(budget, 0)), dtype=torch.int32, device=k.device)
+    _like(seqlens_k, torch.int32, (b,), "seqlens_k")
+    _like(seqlens_out, torch.int32, (b,), "seqlens_out")
+    _like(kept, torch.int32, (b, hk, budget), "kept")
+    _like(weights, torch.float32, (b, hk, caps[0]), "weights")
+    _like(weights_out, torch.float32, (b, hk, caps[1]), "weights_out")
+    for t, what in ((weights, "weights"), (weights_out, "weights_out"), (seqlens_k, "seqlens_k"), (seqlens_out, "seqlens_out"), (kept, "kept")):
+        _dense(t, what)
+    _on(k.device, v, weights, seqlens_k, block_table, k_out, v_out, out_table, weights_out, seqlens_out, kept)
+    blob = pack_flash_evict_args(k, v, k_out, v_out, b, block_table.shape[1] if block_table is not None else 0,
+                                 out_table.shape[1] if out_table is not None else 0, budget, n_sink, n_recent)
+    _call_checked("evict", [k, v, weights, seqlens_k, block_table, k_out, v_out, out_table, weights_out, seqlens_out, kept], blob, k.device, k.dtype, None, stream)
+    return kept, weights_out, seqlens_out

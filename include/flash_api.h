@@ -85,12 +85,68 @@ void run_flash_attn_bwd_bf16(void **tensors, void *extra_args, void *stream);
 void run_flash_attn_kvcache(void **tensors, void *extra_args, void *stream);
 void run_flash_attn_kvcache_bf16(void **tensors, void *extra_args, void *stream);
 
+/* ---- bounded caches: a window with sinks, a cache in pages, eviction by weight ----------------
+ * These have no counterpart in the reference; they follow its calling convention, so that a
+ * `custom` op reaches them like the calls above.
+ *
+ * Attention with a window and sinks, and its gradient.  Row i sees key j when the window's right
+ * side admits it (j <= i + seqlen_k - seqlen_q + right) and either its left side does
+ * (j >= i + seqlen_k - seqlen_q - left) or j < n_sink.  Tensors as run_flash_attn_fwd / _bwd
+ * (rng_state is not read); extra_args (200 bytes): theirs, then i64 n_sink.  p_dropout must be 0,
+ * softmax_scale positive and finite, head_dim a multiple of 8 up to 256.  softmax_lse comes from
+ * unrounded fp32 sums at every head_dim; a row that sees no key gives O = 0, LSE = +inf and no
+ * gradient; a key that no row of a 256-row block sees is not read there.  dq_accum may be NULL. */
+void run_flash_attn_sink_fwd(void **tensors, void *extra_args, void *stream);
+void run_flash_attn_sink_fwd_bf16(void **tensors, void *extra_args, void *stream);
+void run_flash_attn_sink_bwd(void **tensors, void *extra_args, void *stream);
+void run_flash_attn_sink_bwd_bf16(void **tensors, void *extra_args, void *stream);
+
+/* A few query rows over a key/value cache in pages.
+ * tensors: {q, k_pages, v_pages, k_new, v_new, block_table, seqlens_k, o, softmax_lse, weights, weights_out}.
+ *   q, o [b, seqlen_q, h, d]; k_pages, v_pages [num_pages, page_size, h_k, d]; k_new, v_new
+ *   [b, seqlen_knew, h_k, d] (not read when seqlen_knew is 0); block_table int32 [b, max_pages]: row
+ *   j of a sequence is row j % page_size of page block_table[j / page_size] (not read when max_pages
+ *   is 0: a dense cache [b, page_size, h_k, d]); seqlens_k int32 [b]; softmax_lse float [b, h, seqlen_q];
+ *   weights, weights_out float [b, h_k, capacity], capacity = max_pages * page_size (or page_size).
+ * k_new / v_new are written into the cache at rows seqlens_k[i].. (rows behind the capacity are
+ * dropped), then row i of q attends to the rows [0, seqlens_k + seqlen_knew) that a window aligned to
+ * their end, or the sinks, let it see.  A negative length marks an idle sequence (O = 0, LSE = +inf,
+ * nothing written to the cache).  Keys on a page whose number lies outside [0, num_pages) are not
+ * seen, rows that no query row sees are not read.  A page that receives new rows must appear once.
+ * The weights mode is 0 (neither tensor is touched), 1 (weights_out = the attention each key got
+ * from all query rows and heads of its key/value head) or 2 (that on top of `weights`; appended rows
+ * start from 0; weights_out may be weights); rows behind the last key are left as they were.
+ * extra_args (252 bytes): i64 q,k,v,knew,vnew,o batch_stride (of k, v: page stride); the same six
+ * row_strides; the same six head_strides; i64 b, h, h_k, d, seqlen_knew; f32 softmax_scale;
+ * i64 seqlen_q, num_pages, page_size, max_pages, window_size_left, _right, n_sink, weights mode. */
+void run_flash_attn_paged(void **tensors, void *extra_args, void *stream);
+void run_flash_attn_paged_bf16(void **tensors, void *extra_args, void *stream);
+
+/* Eviction: every (sequence, key/value head) keeps at most `budget` rows -- the first n_sink, the last
+ * n_recent and, of those between, the ones of greatest weight (equal weights: the lower row; NaN
+ * below everything) -- which move to the front in their order.
+ * tensors: {k, v, weights, seqlens_k, block_table, k_out, v_out, out_table, weights_out, seqlens_out, kept}.
+ *   Caches and tables as above; kept int32 [b, h_k, budget] receives the row each kept row came from,
+ *   -1 behind the last; seqlens_out[i] = min(seqlens_k[i], budget), a negative length stays.
+ * In place: k_out = k, v_out = v under the same strides and table (weights_out may then be weights, and
+ * seqlens_out may be seqlens_k); otherwise the output cache must not overlap the cache.  Rows and
+ * weights behind the last kept row, and rows of absent pages, are left as they were.
+ * extra_args (192 bytes): i64 k,v,k_out,v_out page_stride; the four row_strides; the four
+ * head_strides; b, h_k, d; num_pages, page_size, max_pages of the cache; the same three of the
+ * output cache; budget, n_sink, n_recent. */
+void run_flash_attn_evict(void **tensors, void *extra_args, void *stream);
+void run_flash_attn_evict_bf16(void **tensors, void *extra_args, void *stream);
+
 /* Error-returning forms of the calls above: 0 on success, a positive hipError_t when a
  * launch failed, -1 when the arguments are unsupported (reason copied to a thread-local
  * buffer readable through flash_attn_last_error()).  dtype: 1 = fp16, 2 = bf16. */
 int flash_attn_fwd_checked(void **tensors, const void *extra_args, int dtype, void *stream);
 int flash_attn_bwd_checked(void **tensors, const void *extra_args, int dtype, void *stream);
 int flash_attn_kvcache_checked(void **tensors, const void *extra_args, int dtype, void *stream);
+int flash_attn_sink_fwd_checked(void **tensors, const void *extra_args, int dtype, void *stream);
+int flash_attn_sink_bwd_checked(void **tensors, const void *extra_args, int dtype, void *stream);
+int flash_attn_paged_checked(void **tensors, const void *extra_args, int dtype, void *stream);
+int flash_attn_evict_checked(void **tensors, const void *extra_args, int dtype, void *stream);
 const char *flash_attn_last_error(void);
 
 /* The same calls with their scratch supplied by the caller, for hosts that own all device
@@ -109,6 +165,16 @@ size_t flash_attn_kvcache_workspace_bytes(const void *extra_args, int dtype);
 int flash_attn_fwd_ws(void **tensors, const void *extra_args, int dtype, void *workspace, size_t workspace_bytes, void *stream);
 int flash_attn_bwd_ws(void **tensors, const void *extra_args, int dtype, void *workspace, size_t workspace_bytes, void *stream);
 int flash_attn_kvcache_ws(void **tensors, const void *extra_args, int dtype, void *workspace, size_t workspace_bytes, void *stream);
+/* the bounded-cache calls: partials of a key split; partial dK / dV and those of the sinks; partials and
+ * the scores behind the weights; nothing */
+size_t flash_attn_sink_fwd_workspace_bytes(const void *extra_args, int dtype);
+size_t flash_attn_sink_bwd_workspace_bytes(const void *extra_args, int dtype, size_t dq_accum_bytes);
+size_t flash_attn_paged_workspace_bytes(const void *extra_args, int dtype);
+size_t flash_attn_evict_workspace_bytes(const void *extra_args, int dtype);
+int flash_attn_sink_fwd_ws(void **tensors, const void *extra_args, int dtype, void *workspace, size_t workspace_bytes, void *stream);
+int flash_attn_sink_bwd_ws(void **tensors, const void *extra_args, int dtype, void *workspace, size_t workspace_bytes, void *stream);
+int flash_attn_paged_ws(void **tensors, const void *extra_args, int dtype, void *workspace, size_t workspace_bytes, void *stream);
+int flash_attn_evict_ws(void **tensors, const void *extra_args, int dtype, void *workspace, size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

@@ -114,6 +114,9 @@ template <typename T> inline T shfl_xor(T v, int mask, int width = 64) {
   return v;
 }
 
+// lanes of a workgroup are fibers of one thread: an LDS atomic is a plain update
+inline unsigned atomicAdd(unsigned *p, unsigned v) { const unsigned old = *p; *p += v; return old; }
+
 // ---- HIP's short vector structs ---------------------------------------------------------------
 struct alignas(8) uint2 { unsigned x, y; };
 struct alignas(16) uint4 { unsigned x, y, z, w; };
@@ -200,6 +203,8 @@ using fa_emu::__float2half_rn;
 using fa_emu::__float2half;
 using fa_emu::__half22float2;
 using fa_emu::hipGetErrorString;
+using fa_emu::atomicAdd;
+using fa_emu::hipErrorOutOfMemory;
 using fa_emu::hipMallocAsync;
 using fa_emu::hipFreeAsync;
 using std::max;

@@ -29,16 +29,17 @@ def lib():
         if not os.path.exists(LIB):
             subprocess.check_call([sys.executable, "-m", "byteir_amd.build", "emu"], cwd=ROOT)
         L = ctypes.CDLL(LIB)
-        for n in ("fwd", "bwd", "kvcache"):
+        for n in ("fwd", "bwd", "kvcache", "sink_fwd", "sink_bwd", "paged", "evict"):
             f = getattr(L, f"flash_attn_{n}_checked")
             f.argtypes = [ctypes.POINTER(_vp), _vp, ctypes.c_int, _vp]
             f.restype = ctypes.c_int
-        for n in ("fwd", "bwd", "kvcache"):
+        for n in ("fwd", "bwd", "kvcache", "sink_fwd", "sink_bwd", "paged", "evict"):
             getattr(L, f"flash_attn_{n}_ws").argtypes = [ctypes.POINTER(_vp), _vp, ctypes.c_int, _vp, ctypes.c_size_t, _vp]
             getattr(L, f"flash_attn_{n}_workspace_bytes").restype = ctypes.c_size_t
-        L.flash_attn_fwd_workspace_bytes.argtypes = [_vp, ctypes.c_int]
-        L.flash_attn_kvcache_workspace_bytes.argtypes = [_vp, ctypes.c_int]
-        L.flash_attn_bwd_workspace_bytes.argtypes = [_vp, ctypes.c_int, ctypes.c_size_t]
+        for n in ("fwd", "kvcache", "sink_fwd", "paged", "evict"):
+            getattr(L, f"flash_attn_{n}_workspace_bytes").argtypes = [_vp, ctypes.c_int]
+        for n in ("bwd", "sink_bwd"):
+            getattr(L, f"flash_attn_{n}_workspace_bytes").argtypes = [_vp, ctypes.c_int, ctypes.c_size_t]
         L.fa_emu_last_error.restype = ctypes.c_char_p
         L.flash_attn_last_error.restype = ctypes.c_char_p
         L.fa_emu_alloc.restype = _vp
@@ -85,8 +86,8 @@ def workspace_bytes(kind, blob, dtype, dq_accum_bytes=0):
     L = lib()
     buf = ctypes.create_string_buffer(blob, len(blob))
     code = 1 if dtype == torch.float16 else 2
-    if kind == "bwd":
-        return L.flash_attn_bwd_workspace_bytes(ctypes.cast(buf, _vp), code, dq_accum_bytes)
+    if kind in ("bwd", "sink_bwd"):
+        return getattr(L, f"flash_attn_{kind}_workspace_bytes")(ctypes.cast(buf, _vp), code, dq_accum_bytes)
     return getattr(L, f"flash_attn_{kind}_workspace_bytes")(ctypes.cast(buf, _vp), code)
 
 
@@ -148,6 +149,42 @@ def kvcache(q, kcache, vcache, knew, vnew, seqlens_k, scale, window=(-1, -1)):
     _call("kvcache", [q, kcache, vcache, knew, vnew, seqlens_k, o, lse],
           ops.pack_flash_kvcache_args(q, kcache, vcache, knew, vnew, o, scale, window), q.dtype)
     return o, lse
+
+
+def sink_fwd(q, k, v, scale, window, n_sink, out=None, workspace=None):
+    from byteir_amd import ops
+    b, sq, h, d = q.shape
+    o, lse = out if out is not None else (torch.empty(q.shape, dtype=q.dtype), torch.empty((b, h, sq), dtype=torch.float32))
+    _call("sink_fwd", [q, k, v, None, o, lse, None], ops.pack_flash_sink_args(q, k, v, o, scale, window, n_sink), q.dtype, workspace)
+    return o, lse
+
+
+def sink_bwd(do, q, k, v, o, lse, scale, window, n_sink, out=None, workspace=None):
+    from byteir_amd import ops
+    b, sq, h, d = q.shape
+    if out is None:
+        like = lambda t: torch.empty_strided(t.shape, t.stride(), dtype=t.dtype)
+        out = (like(q), like(k), like(v), torch.empty((b, h, -(-sq // 128) * 128), dtype=torch.float32))
+    dq, dk, dv, dsm = out
+    _call("sink_bwd", [do, q, k, v, o, lse, None, dq, dk, dv, dsm, None], ops.pack_flash_sink_args(q, k, v, o, scale, window, n_sink), q.dtype, workspace)
+    return dq, dk, dv
+
+
+def paged(q, k_pages, v_pages, table, lens, scale, window, n_sink, k_new=None, v_new=None, weights=None, weights_out=None, out=None, workspace=None):
+    from byteir_amd import ops
+    b, sq, h, d = q.shape
+    o, lse = out if out is not None else (torch.empty(q.shape, dtype=q.dtype), torch.empty((b, h, sq), dtype=torch.float32))
+    mode = 0 if weights_out is None else 1 if weights is None else 2
+    blob = ops.pack_flash_paged_args(q, k_pages, v_pages, k_new, v_new, o, scale, window, n_sink, table.shape[1] if table is not None else 0, mode)
+    _call("paged", [q, k_pages, v_pages, k_new, v_new, table, lens, o, lse, weights, weights_out], blob, q.dtype, workspace)
+    return o, lse
+
+
+def evict(k, v, weights, lens, budget, n_sink, n_recent, table, k_out, v_out, out_table, weights_out, lens_out, kept):
+    from byteir_amd import ops
+    blob = ops.pack_flash_evict_args(k, v, k_out, v_out, lens.shape[0], table.shape[1] if table is not None else 0,
+                                     out_table.shape[1] if out_table is not None else 0, budget, n_sink, n_recent)
+    _call("evict", [k, v, weights, lens, table, k_out, v_out, out_table, weights_out, lens_out, kept], blob, k.dtype)
 
 
 # ---- the reductions, the softmax and the input generator on the host ------------------------
