@@ -113,6 +113,12 @@ def flash_attn():
     return _flash
 
 
+def flash_attn_entry(kind):
+    """flash_attn_<kind>_ws taking the pointer array and the blob as bytes, the rest as integers."""
+    vp = ctypes.c_void_p
+    return ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_char_p, ctypes.c_char_p, ctypes.c_int, vp, ctypes.c_size_t, vp)((f"flash_attn_{kind}_ws", flash_attn()))
+
+
 ALLOC_FN = ctypes.CFUNCTYPE(ctypes.c_void_p, ctypes.c_size_t)
 FREE_FN = ctypes.CFUNCTYPE(None, ctypes.c_void_p)
 OP_LISTENER = ctypes.CFUNCTYPE(None, ctypes.c_void_p, ctypes.c_char_p, ctypes.c_int, ctypes.c_int)

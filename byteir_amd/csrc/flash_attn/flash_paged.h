@@ -14,13 +14,19 @@ struct Pages {
   int shift;
   int64_t k_ps, k_rs, k_hs, v_ps, v_rs, v_hs;  // page, row and head strides (elements)
   FA_HD int capacity() const { return max_pages ? max_pages * page : page; }
-  // page number of a key, and its row there; -1: the page is absent (its number lies outside the pool)
-  __device__ __forceinline__ int locate(int bi, int key, int &row) const {
+  // the table's page number for a key, and the key's row there ...
+  __device__ __forceinline__ int number(int bi, int key, int &row) const {
     if (!max_pages) { row = key; return bi; }
     const int at = (int)(((uint64_t)(uint32_t)key * mul) >> shift);
     row = key - at * page;
-    const int pg = table[(int64_t)bi * max_pages + at];
-    return (unsigned)pg < (unsigned)num_pages ? pg : -1;
+    return table[(int64_t)bi * max_pages + at];
+  }
+  // ... which names a page when it lies inside the pool
+  __device__ __forceinline__ bool present(int pg) const { return (unsigned)pg < (unsigned)num_pages; }
+  // both: the page, or -1 when it is absent
+  __device__ __forceinline__ int locate(int bi, int key, int &row) const {
+    const int pg = number(bi, key, row);
+    return present(pg) ? pg : -1;
   }
 };
 // mul, shift of a page size: mul = ceil(2^shift / page) < 2^32 with shift = 31 + ceil(log2 page),

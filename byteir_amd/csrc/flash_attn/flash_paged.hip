@@ -38,29 +38,19 @@ __global__ void __launch_bounds__(kWaves * 64, D <= 128 ? 2 : 1) paged_kernel(co
   static_assert(kWaveLds >= (D * 32 + 64) * 4, "join buffers must fit the tiles");
   __shared__ __attribute__((aligned(16))) unsigned char lds[kWaves][kWaveLds];
 
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);  // a scalar: units, masks and branches on them are the wave's
   const int r32 = lane & 31, g = lane >> 5;
   const int split = blockIdx.x % p.n_splits;
   const int ct = blockIdx.x / p.n_splits % p.n_ct;
   const int bhk = blockIdx.x / p.n_splits / p.n_ct;
   const int bi = bhk / p.h_k, hk = bhk % p.h_k;
   const int group = p.h / p.h_k, n_cols = group * p.sq;
-  const int sk = p.keys_of(bi);
-
-  const idx::SinkTiles st = p.units(sk, ct);
-  const int n_units = min(st.n, p.max_units), per = p.per_split(n_units);
-  const int u0 = split * per, u1 = min(n_units, u0 + per);
-  if (split > 0 && u0 >= n_units) return;  // whole workgroups
-
-  // column n = ct * 32 + r32 of the S^T tile: query head hk*group + n / sq, query row n % sq
+  // column n = ct * 32 + r32 of the S^T tile: query head hk*group + n / sq, query row n % sq.  Its
+  // fragments are requested before anything that waits for the sequence's length.
   const int n = ct * 32 + r32;
   const bool col_ok = n < n_cols;
   const int qi = col_ok ? n % p.sq : 0, hq = hk * group + (col_ok ? n / p.sq : 0);
-  int lo_lim = 0, hi_lim = 0;
-  if (col_ok) idx::row_limits(p.sq, sk, p.wl, p.wr, qi, lo_lim, hi_lim);
-
-  const T *kg = static_cast<const T *>(p.k) + hk * p.pages.k_hs;
-  const T *vg = static_cast<const T *>(p.v) + hk * p.pages.v_hs;
   vec8 qf[D / 16];
   {
     const T *qg = static_cast<const T *>(p.q) + bi * p.q_bs + (int64_t)qi * p.q_rs + hq * p.q_hs;
@@ -68,52 +58,81 @@ __global__ void __launch_bounds__(kWaves * 64, D <= 128 ? 2 : 1) paged_kernel(co
     for (int ks = 0; ks < D / 16; ++ks)
       qf[ks] = (col_ok && ks * 16 + g * 8 < p.d) ? *reinterpret_cast<const vec8 *>(qg + ks * 16 + g * 8) : vec8{0};
   }
+  const int sk = p.keys_of(bi);
 
+  const idx::SinkTiles st = p.units(sk, ct);
+  const int n_units = min(st.n, p.max_units), per = p.per_split(n_units);
+  const int u0 = split * per, u1 = min(n_units, u0 + per);
+  if (split > 0 && u0 >= n_units) return;  // whole workgroups
+
+  int lo_lim = 0, hi_lim = 0;
+  if (col_ok) idx::row_limits(p.sq, sk, p.wl, p.wr, qi, lo_lim, hi_lim);
+  // what every column of the tile sees: [all_lo, all_hi) and, below it, the sinks
+  int all_lo, all_hi, t0, t1;
+  idx::row_limits(p.sq, sk, p.wl, p.wr, p.sq - 1, all_lo, t0);
+  idx::row_limits(p.sq, sk, p.wl, p.wr, 0, t1, all_hi);
+
+  const T *kg = static_cast<const T *>(p.k) + hk * p.pages.k_hs;
+  const T *vg = static_cast<const T *>(p.v) + hk * p.pages.v_hs;
   T *Kt = reinterpret_cast<T *>(lds[wave]), *Vt = Kt + kUnit * KS;
   uint4 kn[NPV], vn[NPV];
   const int v_c = lane % CPR, v_r = lane / CPR;
   typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
-  // rows from new0 on come from k_new / v_new instead of the cache; the lane that loads one writes
-  // it to the cache (only where every new row is certain to be loaded: p.fuse_append)
+  // rows from new0 on come from k_new / v_new instead of the cache and are written to it
+  // (only where every new row is certain to be visited: p.fuse_append)
   const int new0 = p.fuse_append ? p.seqlens[bi] : 0x7fffffff;
   const T *kng = p.fuse_append ? static_cast<const T *>(p.k_new) + bi * p.kn_bs + hk * p.kn_hs : nullptr;
   const T *vng = p.fuse_append ? static_cast<const T *>(p.v_new) + bi * p.vn_bs + hk * p.vn_hs : nullptr;
-
-  // lane l holds the place of row l % 32 of the unit: its page (-1: nobody sees the row) and its row there
-  int pg_next = -1, row_next = 0, pg = -1;
+  // Where row l % 32 of a unit lies, in lane l: its page number and its row there (-1: nobody sees
+  // the row); requested a unit ahead of the loads that need it.  The number is not looked at
+  // here: a test would wait for it and with it for every load in flight.
+  int pg_next = 0, row_next = -1;
   auto locate = [&](int j) {
     const int key = idx::sink_tile(st, j) * kUnit + r32;
-    pg_next = -1;
-    row_next = 0;
-    if (key < st.hi && (key >= st.lo || key < st.sink)) pg_next = p.pages.locate(bi, key, row_next);
+    row_next = -1;
+    if (key < st.hi && (key >= st.lo || key < st.sink)) pg_next = p.pages.number(bi, key, row_next);
   };
-  auto load_unit = [&](int j) {  // unit j, whose rows locate(j) has found, into the staging registers
+  auto from_lane = [&](int64_t v, int src) {  // lane src's value
+    const int lo = __builtin_amdgcn_ds_bpermute(src * 4, (int)v), hi = __builtin_amdgcn_ds_bpermute(src * 4, (int)(v >> 32));
+    return (int64_t)(((uint64_t)(uint32_t)hi << 32) | (uint32_t)lo);
+  };
+  // The rows of one pass lie on one page when the page size is a multiple of their number: their
+  // address is then a scalar plus an offset that every pass shares, which costs the vector ALU
+  // and the registers nothing.
+  const bool scalar_rows = p.pages.page % RPP == 0 && p.d == D && (uint64_t)p.pages.k_rs < (1 << 26) && (uint64_t)p.pages.v_rs < (1 << 26);
+  const uint32_t k_in = (uint32_t)(v_r * (uint32_t)p.pages.k_rs + v_c * 8), v_in = (uint32_t)(v_r * (uint32_t)p.pages.v_rs + v_c * 8);
+  auto load_unit = [&](int j) -> uint32_t {  // unit j, located, into the staging registers -> which of its rows exist
     const int kv0 = idx::sink_tile(st, j) * kUnit;
-    const int pages = pg_next, rows = row_next;
+    const uint32_t there = (uint32_t)__builtin_amdgcn_ballot_w64(row_next >= 0 && p.pages.present(pg_next));
+    if (there == 0xffffffffu && kv0 + kUnit <= new0 && scalar_rows) {  // a whole unit of the cache
 #pragma unroll
-    for (int s = 0; s < NPV; ++s) {
-      const int src = (s * RPP + v_r) * 4;
-      const int pgr = __builtin_amdgcn_ds_bpermute(src, pages), row = __builtin_amdgcn_ds_bpermute(src, rows);
-      if (pgr >= 0 && v_c * 8 < p.d) {  // columns from head_dim up to D stay zero
-        const int key = kv0 + s * RPP + v_r;
-        const bool fresh = key >= new0;
-        T *kc_row = const_cast<T *>(kg) + (int64_t)pgr * p.pages.k_ps + (int64_t)row * p.pages.k_rs + v_c * 8;
-        T *vc_row = const_cast<T *>(vg) + (int64_t)pgr * p.pages.v_ps + (int64_t)row * p.pages.v_rs + v_c * 8;
-        const T *ks_row = fresh ? kng + (int64_t)(key - new0) * p.kn_rs + v_c * 8 : kc_row;
-        const T *vs_row = fresh ? vng + (int64_t)(key - new0) * p.vn_rs + v_c * 8 : vc_row;
-        const u32x4 a = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(ks_row));
-        const u32x4 b = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(vs_row));
+      for (int s = 0; s < NPV; ++s) {
+        const int64_t pg = __builtin_amdgcn_readlane(pg_next, s * RPP), row = __builtin_amdgcn_readlane(row_next, s * RPP);
+        const u32x4 a = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(kg + pg * p.pages.k_ps + row * p.pages.k_rs + k_in));
+        const u32x4 b = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(vg + pg * p.pages.v_ps + row * p.pages.v_rs + v_in));
         kn[s] = uint4{a.x, a.y, a.z, a.w};
         vn[s] = uint4{b.x, b.y, b.z, b.w};
+      }
+      return there;
+    }
+    const int64_t k_lane = pg_next * p.pages.k_ps + row_next * p.pages.k_rs, v_lane = pg_next * p.pages.v_ps + row_next * p.pages.v_rs;
+#pragma unroll
+    for (int s = 0; s < NPV; ++s) {
+      const int r = s * RPP + v_r, key = kv0 + r;
+      const int64_t ko = from_lane(k_lane, r), vo = from_lane(v_lane, r);
+      kn[s] = uint4{0, 0, 0, 0};  // a row that nobody sees: 0 * finite stays finite in P V
+      vn[s] = uint4{0, 0, 0, 0};
+      if (((there >> r) & 1u) && v_c * 8 < p.d) {  // columns from head_dim up to D stay zero
+        const bool fresh = key >= new0;
+        kn[s] = *reinterpret_cast<const uint4 *>((fresh ? kng + (int64_t)(key - new0) * p.kn_rs : kg + ko) + v_c * 8);
+        vn[s] = *reinterpret_cast<const uint4 *>((fresh ? vng + (int64_t)(key - new0) * p.vn_rs : vg + vo) + v_c * 8);
         if (fresh) {
-          *reinterpret_cast<uint4 *>(kc_row) = kn[s];
-          *reinterpret_cast<uint4 *>(vc_row) = vn[s];
+          *reinterpret_cast<uint4 *>(const_cast<T *>(kg) + ko + v_c * 8) = kn[s];
+          *reinterpret_cast<uint4 *>(const_cast<T *>(vg) + vo + v_c * 8) = vn[s];
         }
-      } else {  // zero rows: 0 * finite stays finite in P V
-        kn[s] = uint4{0, 0, 0, 0};
-        vn[s] = uint4{0, 0, 0, 0};
       }
     }
+    return there;
   };
   auto store_unit = [&]() {
 #pragma unroll
@@ -127,22 +146,28 @@ __global__ void __launch_bounds__(kWaves * 64, D <= 128 ? 2 : 1) paged_kernel(co
   float16v o_acc[D / 32];
 #pragma unroll
   for (int i = 0; i < D / 32; ++i) o_acc[i] = float16v{0};
-  float m_run = -INFINITY, l_run = 0.f;
+  // the reference maximum is raised only when it would grow by more than kSlack (in log2 units), as
+  // in flash_fwd.hip: P stays below 2^kSlack and O is rescaled a few times instead of per unit
+  constexpr float kSlack = 8.f;
+  float m_run = -INFINITY, m_scaled = 0.f, l_run = 0.f;
   const float c = p.scale_log2;
 
+  uint32_t there = 0;
   if (u0 + wave < u1) {
     locate(u0 + wave);
-    load_unit(u0 + wave);
-    pg = pg_next;
+    there = load_unit(u0 + wave);
     if (u0 + wave + kWaves < u1) locate(u0 + wave + kWaves);
     store_unit();
   }
+  // The Q fragments are consumed here: the wait for their loads would otherwise stand before the first
+  // MFMA of every unit and drain the loads of the next one too.
+#pragma unroll
+  for (int ks = 0; ks < D / 16; ++ks) FA_PIN(qf[ks]);
   for (int j = u0 + wave; j < u1; j += kWaves) {
     const bool has_next = j + kWaves < u1;
-    const uint32_t there = (uint32_t)__builtin_amdgcn_ballot_w64(pg >= 0);  // rows of unit j that were read
+    uint32_t there_next = 0;
     if (has_next) {
-      load_unit(j + kWaves);
-      pg = pg_next;
+      there_next = load_unit(j + kWaves);
       if (j + 2 * kWaves < u1) locate(j + 2 * kWaves);
     }
     float16v s = float16v{0};
@@ -150,10 +175,12 @@ __global__ void __launch_bounds__(kWaves * 64, D <= 128 ? 2 : 1) paged_kernel(co
     for (int ks = 0; ks < D / 16; ++ks)
       s = Traits<T>::mfma(lds_read8<T>(&Kt[r32 * KS + ks * 16 + g * 8]), qf[ks], s);
     const int kv0 = idx::sink_tile(st, j) * kUnit;
+    if (there != 0xffffffffu || kv0 + kUnit > all_hi || (kv0 < all_lo && kv0 + kUnit > p.n_sink)) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int r = (i >> 2) * 8 + g * 4 + (i & 3), kv = kv0 + r;
-      if (kv >= hi_lim || (kv < lo_lim && kv >= p.n_sink) || !((there >> r) & 1u)) s[i] = -INFINITY;
+      for (int i = 0; i < 16; ++i) {
+        const int r = (i >> 2) * 8 + g * 4 + (i & 3), kv = kv0 + r;
+        if (kv >= hi_lim || (kv < lo_lim && kv >= p.n_sink) || !((there >> r) & 1u)) s[i] = -INFINITY;
+      }
     }
     if constexpr (Scores) {
       if (col_ok) {
@@ -163,14 +190,23 @@ __global__ void __launch_bounds__(kWaves * 64, D <= 128 ? 2 : 1) paged_kernel(co
           *reinterpret_cast<float4 *>(sp + i4 * 8) = float4{s[i4 * 4], s[i4 * 4 + 1], s[i4 * 4 + 2], s[i4 * 4 + 3]};
       }
     }
-    float mx = -INFINITY;
+    float mx = s[0];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[i]);
-    mx = fmaxf(mx, partner32(mx));
-    const float m_new = fmaxf(m_run, mx);
-    const float m_use = m_new == -INFINITY ? 0.f : m_new;
-    const float alpha = exp2_fast((m_run - m_use) * c);
-    const float m_scaled = m_use * c;
+    for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
+    // +inf for the first finite score of a column, NaN (false) for -inf - -inf
+    if (__builtin_amdgcn_ballot_w64((mx - m_run) * c > kSlack) != 0) {
+      mx = fmaxf(mx, partner32(mx));
+      const float m_new = (mx - m_run) * c > kSlack ? mx : m_run;
+      const float m_use = m_new == -INFINITY ? 0.f : m_new;
+      const float alpha = exp2_fast((m_run - m_use) * c);
+      l_run *= alpha;
+      m_run = m_new;
+      m_scaled = m_use * c;
+#pragma unroll
+      for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o_acc[db][i] *= alpha;
+    }
     float rs = 0.f;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
@@ -178,12 +214,7 @@ __global__ void __launch_bounds__(kWaves * 64, D <= 128 ? 2 : 1) paged_kernel(co
       s[i] = e;
       rs += e;
     }
-    l_run = l_run * alpha + rs;
-    m_run = m_new;
-#pragma unroll
-    for (int db = 0; db < D / 32; ++db)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) o_acc[db][i] *= alpha;
+    l_run += rs;
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
       float pf[8];
@@ -195,6 +226,7 @@ __global__ void __launch_bounds__(kWaves * 64, D <= 128 ? 2 : 1) paged_kernel(co
         o_acc[db] = Traits<T>::mfma(lds_read_operand_tr<T>(Vt, VS, w * 16, db * 32), pb, o_acc[db]);
     }
     if (has_next) store_unit();  // after every read of unit j in program order
+    there = there_next;
   }
 
   // ---- the four waves' partials joined through LDS (each wave writes into its own region) ----
@@ -230,13 +262,18 @@ __global__ void __launch_bounds__(kWaves * 64, D <= 128 ? 2 : 1) paged_kernel(co
   T *og = static_cast<T *>(p.o) + bi * p.o_bs + (int64_t)oi * p.o_rs + oh * p.o_hs;
   const int64_t prow = (((int64_t)split * p.b + bi) * p.h + oh) * p.sq + oi;
 #pragma unroll
-  for (int x = 0; x < D / 8; ++x) {
+  for (int x = 0; x < D / 8; x += 4) {
     const int dcol = slice * (D / 8) + x;
-    float acc = 0.f;
+    float acc[4];
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) acc += wgt[w] * reinterpret_cast<const float *>(lds[w])[dcol * 32 + on];
-    if (!final_pass) p.o_part[prow * D + dcol] = acc;
-    else if (dcol < p.d) og[dcol] = (T)(acc * inv);
+    for (int y = 0; y < 4; ++y) {
+      acc[y] = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) acc[y] += wgt[w] * reinterpret_cast<const float *>(lds[w])[(dcol + y) * 32 + on];
+    }
+    typedef T vec4 __attribute__((ext_vector_type(4)));
+    if (!final_pass) *reinterpret_cast<float4 *>(p.o_part + prow * D + dcol) = float4{acc[0], acc[1], acc[2], acc[3]};
+    else if (dcol < p.d) *reinterpret_cast<vec4 *>(og + dcol) = vec4{(T)(acc[0] * inv), (T)(acc[1] * inv), (T)(acc[2] * inv), (T)(acc[3] * inv)};
   }
   if (slice == 0) {
     if (final_pass) p.lse[((int64_t)bi * p.h + oh) * p.sq + oi] = empty ? INFINITY : m_all * p.scale + log2_fast(l_all) * kLn2;
@@ -392,8 +429,11 @@ hipError_t launch_paged(PagedParams &p, int dtype, hipStream_t stream) {
     units = std::min<int64_t>(units, (std::min(p.n_sink, cap) + kUnit - 1) / kUnit + ((int64_t)p.wl + p.sq + kUnit) / kUnit + 2);
   p.max_units = (int)std::max<int64_t>(units, 1);
   const int64_t base = (int64_t)p.b * p.h_k * p.n_ct;
-  p.min_units = kWaves;
-  p.n_splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>((1024 + base - 1) / base, 64), p.max_units / (2 * kWaves)));
+  // Splits: enough workgroups that unequal sequences even out (8 for every CU, two of them at a time),
+  // of at least 512 keys each when there are many and 128 (a unit a wave) when there are few
+  const int64_t want = std::max<int64_t>(1, 2048 / base);
+  p.min_units = (int)std::min<int64_t>(16, std::max<int64_t>(kWaves, p.max_units / want));
+  p.n_splits = p.max_units <= 2 * kWaves ? 1 : (int)std::min<int64_t>(64, (p.max_units + p.min_units - 1) / p.min_units);
   // the attention kernel appends when one workgroup's tile covers all columns and its window reaches the first new row
   p.fuse_append = p.n_new > 0 && p.n_ct == 1 && (p.wl < 0 || p.n_new <= (int64_t)p.sq + p.wl);
   return dtype == 1 ? paged_t<_Float16>(p, stream) : paged_t<__bf16>(p, stream);

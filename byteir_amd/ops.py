@@ -5,7 +5,9 @@ HIP kernel reached through libbrt_rocm_kernels.so / libflash_attn.so.  Shapes fo
 reference's op kernels: reductions take the canonical [A, B, C] view computed by
 `canonicalize_reduce` (ReduceImpl, runtime/lib/backends/cuda/providers/default/reduction/reduce_impl.h:28-59).
 """
+import collections
 import ctypes
+import functools
 import struct
 
 import torch
@@ -279,13 +281,38 @@ def flash_attn_kvcache(q, kcache, vcache, knew, vnew, seqlens_k, scale, window=(
 
 
 # ---- attention with a window and sinks, over a paged cache, and eviction from a cache -----------
-def _on(device, *tensors):
-    """Every tensor given lies on `device` (a GPU)."""
-    if device.type != "cuda":
+# A call is checked, its blob packed and its scratch asked for once per set of shapes, strides, types
+# and scalars (the _plan_* functions, memoised on exactly those: nothing of a tensor's contents or
+# address); what is left per call is the outputs, the pointers and the launch.  One decode step or
+# short prompt takes the GPU 10-15 us, checks and packing took the host 25-45 us.
+_PLANS = 4096  # plans kept; serving sees one per batch shape, training one per sequence length
+_Sig = collections.namedtuple("_Sig", "shape stride dtype device")
+
+
+def _sig(t):
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.get_device())
+
+
+def _fresh(shape, dtype, device):
+    """The signature of a dense tensor that the call itself makes."""
+    stride, n = [], 1
+    for x in reversed(shape):
+        stride.insert(0, n)
+        n *= max(x, 1)
+    return _Sig(torch.Size(shape), tuple(stride), dtype, device)
+
+
+def _sigs(*sigs):
+    return [None if s is None else _Sig(*s) for s in sigs]
+
+
+def _on(device, *sigs):
+    """Everything lies on one GPU."""
+    if device < 0:
         raise ValueError("device tensor required: the ROCm provider has no host path")
-    for t in tensors:
+    for t in sigs:
         if t is not None and t.device != device:
-            raise ValueError(f"tensors on {device} and {t.device}: one call takes tensors of one GPU")
+            raise ValueError(f"tensors on devices {device} and {t.device}: one call takes tensors of one GPU")
 
 
 def _like(t, dtype, shape, what):
@@ -294,54 +321,86 @@ def _like(t, dtype, shape, what):
 
 
 def _dense(t, what):
-    if t is not None and not t.is_contiguous():
-        raise ValueError(f"{what} must be dense row-major")
+    n = 1
+    for size, stride in zip(reversed(t.shape), reversed(t.stride)) if t is not None and 0 not in t.shape else ():
+        if size != 1 and stride != n:
+            raise ValueError(f"{what} must be dense row-major")
+        n *= size
 
 
-def _half(q, *tensors):
+def _half(q, *sigs):
     if q.dtype not in (torch.float16, torch.bfloat16):
         raise ValueError(f"{q.dtype} is not supported (float16 or bfloat16)")
-    for t in tensors:
+    for t in sigs:
         if t is not None and t.dtype != q.dtype:
             raise ValueError(f"tensors of {q.dtype} and {t.dtype}: one call takes one storage type")
-    for t in (q,) + tensors:
-        if t is not None and (t.dim() != 4 or (t.numel() and t.stride(3) != 1)):
+    for t in (q,) + sigs:
+        if t is not None and (len(t.shape) != 4 or (0 not in t.shape and t.shape[3] > 1 and t.stride[3] != 1)):
             raise ValueError("4-d tensors with a dense head_dim required")
 
 
 def _strides(t):
     """(outer, row, head) strides; an axis of length 1 has none that counts."""
-    return [t.stride(i) if t.shape[i] > 1 else 0 for i in range(3)] if t is not None else [0, 0, 0]
+    return [t.stride[i] if t.shape[i] > 1 else 0 for i in range(3)] if t is not None else [0, 0, 0]
 
 
 def _overlaps(t):
     """Whether elements of a view may share memory (an expanded axis, say)."""
     end = 0
-    for stride, n in sorted((t.stride(i), t.shape[i]) for i in range(t.dim()) if t.shape[i] > 1):
+    for stride, n in sorted((s, n) for s, n in zip(t.stride, t.shape) if n > 1):
         if stride <= end:
             return True
         end += stride * (n - 1)
     return False
 
 
-def _call_checked(kind, tensors, blob, device, dtype, workspace, stream, dq_accum_bytes=0):
-    """flash_attn_<kind>_ws on the tensors' own GPU, with the caller's scratch or scratch from torch's
+def _plan(kind, dtype, blob, dq_accum_bytes=0):
+    """What a call needs besides pointers: (entry point, blob, storage type, scratch bytes)."""
+    return _lib.flash_attn_entry(kind), blob, 1 if dtype == torch.float16 else 2, flash_attn_workspace_bytes(kind, dtype, blob, dq_accum_bytes)
+
+
+_pack11 = struct.Struct("11P").pack
+_pack12 = struct.Struct("12P").pack
+
+
+def _ptr(t):
+    return 0 if t is None else t.data_ptr()
+
+
+def _on_stream(fn):
+    """Runs a call with stream=... under that stream, so that what it allocates belongs to it."""
+    @functools.wraps(fn)
+    def call(*args, stream=None, **kw):
+        if stream is None:
+            return fn(*args, **kw)
+        first = args[0] if args else kw[fn.__code__.co_varnames[0]]
+        if stream.device != first.device:
+            raise ValueError(f"a stream of {stream.device} for tensors of {first.device}")
+        with torch.cuda.stream(stream):
+            return fn(*args, **kw)
+    return call
+
+
+def _launch(plan, tensors, on, workspace):
+    """The call on the GPU of `on` and its current stream, with the caller's scratch or scratch from torch's
     allocator; raises ValueError for a call that the library refuses."""
-    with torch.cuda.device(device):
-        stream = stream if stream is not None else torch.cuda.current_stream()
-        if workspace is None:
-            need = flash_attn_workspace_bytes(kind, dtype, blob, dq_accum_bytes)
-            if need:
-                workspace = torch.empty(need, dtype=torch.uint8, device=device)
-                workspace.record_stream(stream)
-        _call_custom_ws(kind, dtype, tensors, blob, workspace, stream)
-
-
-def _check_sink(q, k, v, o):
-    _half(q, k, v, o)
-    b, sq, h, d = q.shape
-    if k.shape != v.shape or k.shape[0] != b or k.shape[3] != d:
-        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not fit together")
+    entry, blob, code, need = plan
+    device = on.get_device()
+    if torch.cuda.current_device() != device:
+        with torch.cuda.device(device):
+            return _launch(plan, tensors, on, workspace)
+    ws, n = 0, 0
+    if workspace is not None:
+        if workspace.get_device() != device:
+            raise ValueError("the workspace must lie on the tensors' GPU")
+        ws, n = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    elif need:
+        workspace = torch.empty(need, dtype=torch.uint8, device=on.device)
+        ws, n = workspace.data_ptr(), need
+    rc = entry(tensors, blob, code, ws, n, torch.cuda.current_stream().cuda_stream)
+    if rc < 0:
+        raise ValueError(_lib.flash_attn().flash_attn_last_error().decode())
+    _lib.check(rc, "flash_attn")
 
 
 def pack_flash_sink_args(q, k, v, o, scale, window, n_sink):
@@ -349,60 +408,101 @@ def pack_flash_sink_args(q, k, v, o, scale, window, n_sink):
     return pack_flash_args(q, k, v, o, scale, window) + struct.pack("<q", n_sink)
 
 
-def flash_attn_sink_fwd(q, k, v, scale, window=(-1, 0), n_sink=0, stream=None, out=None, workspace=None):
+def _sink_blob(q, k, v, o, scale, window, n_sink):
+    """pack_flash_sink_args from signatures."""
+    _half(q, k, v, o)
+    b, sq, h, d = q.shape
+    sk = k.shape[1]
+    if k.shape != v.shape or k.shape[0] != b or k.shape[3] != d:
+        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not fit together")
+    _like(o, q.dtype, q.shape, "o")
+    each = [_strides(t) for t in (q, k, v, o)]
+    return (struct.pack("<17q", *[s[i] for i in range(3) for s in each], b, h, k.shape[2], d, round_up(d, 32)) + struct.pack("<f", scale)
+            + struct.pack("<4q", sq, sk, round_up(sq, 128), round_up(sk, 128)) + struct.pack("<f", 0.0) + struct.pack("<3q", *window, n_sink))
+
+
+@functools.lru_cache(_PLANS)
+def _plan_sink_fwd(q, k, v, o, lse, scale, window, n_sink):
+    q, k, v, o, lse = _sigs(q, k, v, o, lse)
+    _half(q)
+    b, sq, h, _ = q.shape
+    o = o or _fresh(q.shape, q.dtype, q.device)
+    lse = lse or _fresh((b, h, sq), torch.float32, q.device)
+    blob = _sink_blob(q, k, v, o, scale, window, n_sink)
+    _like(lse, torch.float32, (b, h, sq), "lse")
+    _dense(lse, "lse")
+    if _overlaps(o):
+        raise ValueError("o must not be a broadcast view")
+    _on(q.device, k, v, o, lse)
+    return _plan("sink_fwd", q.dtype, blob)
+
+
+@_on_stream
+def flash_attn_sink_fwd(q, k, v, scale, window=(-1, 0), n_sink=0, out=None, workspace=None):
     """Attention in which row i sees the keys of its window, as in flash_attn_fwd, and of the first
     `n_sink` keys those that the window's right side admits: q [b, sq, h, d], k, v [b, sk, h_k, d]
     -> (o [b, sq, h, d], lse [b, h, sq] f32).  lse comes from unrounded fp32 sums at every
     head_dim.  A row that sees no key gives o = 0, lse = +inf.  A key that no row of a 256-row
     block sees may hold anything; a NaN in a key that some row sees may reach the rows beside it.
     out: optional (o, lse) to write into; workspace: optional uint8 device tensor of
-    flash_attn_workspace_bytes("sink_fwd", ...) bytes."""
-    _check_sink(q, k, v, None)
-    b, sq, h, d = q.shape
-    o, lse = out if out is not None else (torch.empty((b, sq, h, d), dtype=q.dtype, device=q.device),
-                                          torch.empty((b, h, sq), dtype=torch.float32, device=q.device))
-    _half(q, o)
-    _like(o, q.dtype, q.shape, "o")
-    _like(lse, torch.float32, (b, h, sq), "lse")
-    _dense(lse, "lse")
-    _on(q.device, k, v, o, lse, workspace)
-    _call_checked("sink_fwd", [q, k, v, None, o, lse, None], pack_flash_sink_args(q, k, v, o, scale, window, n_sink), q.device, q.dtype, workspace, stream)
+    flash_attn_workspace_bytes("sink_fwd", ...) bytes; stream: runs there, not on the current stream
+    (these three are keywords of the calls below too)."""
+    o, lse = out if out is not None else (None, None)
+    plan = _plan_sink_fwd(_sig(q), _sig(k), _sig(v), _sig(o), _sig(lse), scale, tuple(window), n_sink)
+    if out is None:
+        b, sq, h, _ = q.shape
+        o, lse = torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty((b, h, sq), dtype=torch.float32, device=q.device)
+    _launch(plan, _pack11(q.data_ptr(), k.data_ptr(), v.data_ptr(), 0, o.data_ptr(), lse.data_ptr(), 0, 0, 0, 0, 0), q, workspace)
     return o, lse
 
 
-def flash_attn_sink_bwd(dout, q, k, v, o, lse, scale, window=(-1, 0), n_sink=0, stream=None, out=None, workspace=None):
-    """Gradients of flash_attn_sink_fwd -> (dq, dk, dv), laid out as q, k, v (densely where one is a
-    broadcast view); dk and dv of a
-    key/value head are the sums over its query heads.  o and lse are the forward call's.
-    out: optional (dq, dk, dv, d_softmax, dq_accum, _) of flash_attn_bwd_buffers."""
-    _check_sink(q, k, v, o)
+@functools.lru_cache(_PLANS)
+def _plan_sink_bwd(dout, q, k, v, o, lse, dq, dk, dv, dsm, dq_accum, scale, window, n_sink):
+    """-> None when dout has to be laid out as o, or a broadcast input densely, before the call."""
+    dout, q, k, v, o, lse, dq, dk, dv, dsm, dq_accum = _sigs(dout, q, k, v, o, lse, dq, dk, dv, dsm, dq_accum)
+    blob = _sink_blob(q, k, v, o, scale, window, n_sink)
     _half(q, dout)
     b, sq, h, d = q.shape
-    _like(o, q.dtype, q.shape, "o")
     _like(dout, q.dtype, q.shape, "dout")
     _like(lse, torch.float32, (b, h, sq), "lse")
     _dense(lse, "lse")
-    if _strides(dout) != _strides(o):  # the library addresses dout with the strides of o
-        dout = torch.empty_strided(o.shape, o.stride(), dtype=o.dtype, device=o.device).copy_(dout)
-    # gradients are written with the strides of q, k, v: a broadcast one is laid out densely first
-    q, k, v = (t.contiguous() if _overlaps(t) else t for t in (q, k, v))
-    if out is None:
-        like = lambda t: torch.empty_strided(t.shape, t.stride(), dtype=t.dtype, device=t.device)
-        # the grouped heads' partials go into the workspace, not into a dq_accum tensor
-        out = (like(q), like(k), like(v), torch.empty((b, h, round_up(sq, 128)), dtype=torch.float32, device=q.device), None, None)
-    dq, dk, dv, dsm, dq_accum, _ = out
-    for g, t, what in ((dq, q, "dq"), (dk, k, "dk"), (dv, v, "dv")):
-        _like(g, t.dtype, t.shape, what)
-        if _strides(g) != _strides(t):
-            raise ValueError(f"{what} must be laid out as {what[1:]}")
-    _like(dsm, torch.float32, (b, h, round_up(sq, 128)), "d_softmax")
-    _dense(dsm, "d_softmax")
-    if dq_accum is not None:
+    _on(q.device, dout, k, v, o, lse)
+    if _strides(dout) != _strides(o) or any(_overlaps(t) for t in (q, k, v)):
+        return None
+    if dq is not None:
+        for g, t, what in ((dq, q, "dq"), (dk, k, "dk"), (dv, v, "dv")):
+            _like(g, t.dtype, t.shape, what)
+            if _strides(g) != _strides(t):
+                raise ValueError(f"{what} must be laid out as {what[1:]}")
+        _like(dsm, torch.float32, (b, h, round_up(sq, 128)), "d_softmax")
+        _dense(dsm, "d_softmax")
         _like(dq_accum, torch.float32, (b, round_up(sq, 128), h, round_up(d, 32)), "dq_accum")
         _dense(dq_accum, "dq_accum")
-    _on(q.device, dout, k, v, o, lse, dq, dk, dv, dsm, dq_accum, workspace)
-    _call_checked("sink_bwd", [dout, q, k, v, o, lse, None, dq, dk, dv, dsm, dq_accum], pack_flash_sink_args(q, k, v, o, scale, window, n_sink),
-                  q.device, q.dtype, workspace, stream, dq_accum.numel() * 4 if dq_accum is not None else 0)
+        _on(q.device, dq, dk, dv, dsm, dq_accum)
+    accum = 4 * b * round_up(sq, 128) * h * round_up(d, 32) if dq_accum is not None else 0
+    return _plan("sink_bwd", q.dtype, blob, accum)
+
+
+@_on_stream
+def flash_attn_sink_bwd(dout, q, k, v, o, lse, scale, window=(-1, 0), n_sink=0, out=None, workspace=None):
+    """Gradients of flash_attn_sink_fwd -> (dq, dk, dv), laid out as q, k, v (densely where one is a
+    broadcast view); dk and dv of a key/value head are the sums over its query heads.  o and lse
+    are the forward call's.  out: optional (dq, dk, dv, d_softmax, dq_accum, _) of
+    flash_attn_bwd_buffers; without it the partial sums of grouped heads go into the workspace."""
+    dq, dk, dv, dsm, dq_accum, _ = out if out is not None else (None,) * 6
+    key = (_sig(lse), _sig(dq), _sig(dk), _sig(dv), _sig(dsm), _sig(dq_accum), scale, tuple(window), n_sink)
+    plan = _plan_sink_bwd(_sig(dout), _sig(q), _sig(k), _sig(v), _sig(o), *key)
+    if plan is None:
+        # the library addresses dout with the strides of o, and the gradients with those of q, k, v
+        o, q, k, v = (t.contiguous() if _overlaps(_Sig(*_sig(t))) else t for t in (o, q, k, v))
+        if _strides(_Sig(*_sig(dout))) != _strides(_Sig(*_sig(o))):
+            dout = torch.empty_strided(o.shape, o.stride(), dtype=o.dtype, device=o.device).copy_(dout)
+        plan = _plan_sink_bwd(_sig(dout), _sig(q), _sig(k), _sig(v), _sig(o), *key)
+    if out is None:
+        dq, dk, dv = (torch.empty_strided(t.shape, t.stride(), dtype=t.dtype, device=t.device) for t in (q, k, v))
+        dsm = torch.empty((q.shape[0], q.shape[2], round_up(q.shape[1], 128)), dtype=torch.float32, device=q.device)
+    _launch(plan, _pack12(dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), 0, dq.data_ptr(), dk.data_ptr(),
+                          dv.data_ptr(), dsm.data_ptr(), _ptr(dq_accum)), q, workspace)
     return dq, dk, dv
 
 
@@ -411,6 +511,10 @@ def pack_flash_paged_args(q, k_pages, v_pages, k_new, v_new, o, scale, window, n
     caches' outer stride is that of a page), i64 b, h, h_k, d, seqlen_knew; f32 scale; i64 seqlen_q,
     num_pages, page_size, max_pages, window left, right, n_sink, weights (0 none, 1 from zero, 2 on top
     of weights)."""
+    return _paged_blob(*_sigs(*(_sig(t) for t in (q, k_pages, v_pages, k_new, v_new, o))), scale, window, n_sink, max_pages, weights)
+
+
+def _paged_blob(q, k_pages, v_pages, k_new, v_new, o, scale, window, n_sink, max_pages, weights):
     b, sq, h, d = q.shape
     each = [_strides(t) for t in (q, k_pages, v_pages, k_new, v_new, o)]
     ints1 = [s[i] for i in range(3) for s in each] + [b, h, k_pages.shape[2], d, k_new.shape[1] if k_new is not None else 0]
@@ -418,8 +522,57 @@ def pack_flash_paged_args(q, k_pages, v_pages, k_new, v_new, o, scale, window, n
     return struct.pack("<23q", *ints1) + struct.pack("<f", scale) + struct.pack("<8q", *ints2)
 
 
+def _table(t, pages, b, what):
+    """Checks a block table (or its absence) -> (max_pages, rows a sequence can hold)."""
+    if t is None:
+        if pages.shape[0] != b:
+            raise ValueError(f"{b} sequences, but a dense cache of {pages.shape[0]}")
+        return 0, pages.shape[1]
+    if len(t.shape) != 2 or t.shape[1] == 0:
+        raise ValueError(f"{what} must be [b, max_pages] with at least one page")
+    _like(t, torch.int32, (b, t.shape[1]), what)
+    _dense(t, what)
+    return t.shape[1], t.shape[1] * pages.shape[1]
+
+
+@functools.lru_cache(_PLANS)
+def _plan_paged(q, k_pages, v_pages, block_table, seqlens_k, k_new, v_new, weights, weights_out, o, lse, scale, window, n_sink):
+    q, k_pages, v_pages, block_table, seqlens_k, k_new, v_new, weights, weights_out, o, lse = _sigs(
+        q, k_pages, v_pages, block_table, seqlens_k, k_new, v_new, weights, weights_out, o, lse)
+    _half(q, k_pages, v_pages, k_new, v_new, o)
+    b, sq, h, d = q.shape
+    hk = k_pages.shape[2]
+    if k_pages.shape != v_pages.shape or k_pages.shape[3] != d:
+        raise ValueError(f"q {tuple(q.shape)}, k_pages {tuple(k_pages.shape)} and v_pages {tuple(v_pages.shape)} do not fit together")
+    if (k_new is None) != (v_new is None):
+        raise ValueError("k_new and v_new must be given together")
+    if k_new is not None:
+        if _overlaps(k_pages) or _overlaps(v_pages):
+            raise ValueError("new rows cannot be written to a broadcast view")
+        for t in (k_new, v_new):
+            _like(t, q.dtype, (b, k_new.shape[1], hk, d), "k_new / v_new")
+    if weights is not None and weights_out is None:
+        raise ValueError("weights without weights_out")
+    max_pages, cap = _table(block_table, k_pages, b, "block_table")
+    _like(seqlens_k, torch.int32, (b,), "seqlens_k")
+    o = o or _fresh(q.shape, q.dtype, q.device)
+    lse = lse or _fresh((b, h, sq), torch.float32, q.device)
+    _like(o, q.dtype, q.shape, "o")
+    if _overlaps(o):
+        raise ValueError("o must not be a broadcast view")
+    _like(lse, torch.float32, (b, h, sq), "lse")
+    for t, what in ((weights, "weights"), (weights_out, "weights_out")):
+        _like(t, torch.float32, (b, hk, cap), what)
+    for t, what in ((weights, "weights"), (weights_out, "weights_out"), (lse, "lse"), (seqlens_k, "seqlens_k")):
+        _dense(t, what)
+    _on(q.device, k_pages, v_pages, k_new, v_new, block_table, seqlens_k, o, lse, weights, weights_out)
+    mode = 0 if weights_out is None else 1 if weights is None else 2
+    return _plan("paged", q.dtype, _paged_blob(q, k_pages, v_pages, k_new, v_new, o, scale, window, n_sink, max_pages, mode))
+
+
+@_on_stream
 def flash_attn_paged(q, k_pages, v_pages, block_table, seqlens_k, scale, window=(-1, 0), n_sink=0, k_new=None, v_new=None, weights=None,
-                     weights_out=None, stream=None, out=None, workspace=None):
+                     weights_out=None, out=None, workspace=None):
     """Attention of a few query rows over a key/value cache in pages.  q [b, sq, h, d]; k_pages, v_pages
     [num_pages, page_size, h_k, d]; block_table int32 [b, max_pages]: row j of sequence i is row
     j % page_size of page block_table[i][j // page_size].  block_table None: a dense cache
@@ -435,44 +588,14 @@ def flash_attn_paged(q, k_pages, v_pages, block_table, seqlens_k, scale, window=
     attention that key j got from all query rows and heads of key/value head c, for the rows j in
     the cache after the call; the others are left as they were.
     -> (o, lse[b, h, sq] f32), and weights_out when given."""
-    _half(q, k_pages, v_pages, k_new, v_new)
-    b, sq, h, d = q.shape
-    hk = k_pages.shape[2]
-    if k_pages.shape != v_pages.shape or k_pages.shape[3] != d:
-        raise ValueError(f"q {tuple(q.shape)}, k_pages {tuple(k_pages.shape)} and v_pages {tuple(v_pages.shape)} do not fit together")
-    if (k_new is None) != (v_new is None):
-        raise ValueError("k_new and v_new must be given together")
-    if k_new is not None:
-        if _overlaps(k_pages) or _overlaps(v_pages):
-            raise ValueError("new rows cannot be written to a broadcast view")
-        for t in (k_new, v_new):
-            _like(t, q.dtype, (b, k_new.shape[1], hk, d), "k_new / v_new")
-    if weights is not None and weights_out is None:
-        raise ValueError("weights without weights_out")
-    max_pages = 0
-    if block_table is not None:
-        if block_table.dim() != 2 or block_table.shape[1] == 0:
-            raise ValueError("block_table must be [b, max_pages] with at least one page")
-        _like(block_table, torch.int32, (b, block_table.shape[1]), "block_table")
-        max_pages = block_table.shape[1]
-    elif k_pages.shape[0] != b:
-        raise ValueError(f"{b} sequences, but a dense cache of {k_pages.shape[0]}")
-    cap = (max_pages or 1) * k_pages.shape[1]
-    _like(seqlens_k, torch.int32, (b,), "seqlens_k")
-    o, lse = out if out is not None else (torch.empty((b, sq, h, d), dtype=q.dtype, device=q.device),
-                                          torch.empty((b, h, sq), dtype=torch.float32, device=q.device))
-    _half(q, o)
-    _like(o, q.dtype, q.shape, "o")
-    _like(lse, torch.float32, (b, h, sq), "lse")
-    for t, what in ((weights, "weights"), (weights_out, "weights_out")):
-        _like(t, torch.float32, (b, hk, cap), what)
-        _dense(t, what)
-    for t, what in ((lse, "lse"), (block_table, "block_table"), (seqlens_k, "seqlens_k")):
-        _dense(t, what)
-    _on(q.device, k_pages, v_pages, k_new, v_new, block_table, seqlens_k, o, lse, weights, weights_out, workspace)
-    mode = 0 if weights_out is None else 1 if weights is None else 2
-    blob = pack_flash_paged_args(q, k_pages, v_pages, k_new, v_new, o, scale, window, n_sink, max_pages, mode)
-    _call_checked("paged", [q, k_pages, v_pages, k_new, v_new, block_table, seqlens_k, o, lse, weights, weights_out], blob, q.device, q.dtype, workspace, stream)
+    o, lse = out if out is not None else (None, None)
+    plan = _plan_paged(_sig(q), _sig(k_pages), _sig(v_pages), _sig(block_table), _sig(seqlens_k), _sig(k_new), _sig(v_new), _sig(weights),
+                       _sig(weights_out), _sig(o), _sig(lse), scale, tuple(window), n_sink)
+    if out is None:
+        b, sq, h, _ = q.shape
+        o, lse = torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty((b, h, sq), dtype=torch.float32, device=q.device)
+    _launch(plan, _pack11(q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_new), _ptr(v_new), _ptr(block_table), seqlens_k.data_ptr(),
+                          o.data_ptr(), lse.data_ptr(), _ptr(weights), _ptr(weights_out)), q, workspace)
     return (o, lse) if weights_out is None else (o, lse, weights_out)
 
 
@@ -480,13 +603,47 @@ def pack_flash_evict_args(k, v, k_out, v_out, b, max_pages, max_pages_out, budge
     """The 192-byte extra_args blob of flash_attn_evict, 24 i64: the outer (page), row and head strides of k, v,
     k_out, v_out; b, h_k, d; num_pages, page_size, max_pages of the cache and of the output cache; budget,
     n_sink, n_recent."""
+    return _evict_blob(*_sigs(_sig(k), _sig(v), _sig(k_out), _sig(v_out)), b, max_pages, max_pages_out, budget, n_sink, n_recent)
+
+
+def _evict_blob(k, v, k_out, v_out, b, max_pages, max_pages_out, budget, n_sink, n_recent):
     each = [_strides(t) for t in (k, v, k_out, v_out)]
     return struct.pack("<24q", *[s[i] for i in range(3) for s in each], b, k.shape[2], k.shape[3], k.shape[0], k.shape[1], max_pages,
                        k_out.shape[0], k_out.shape[1], max_pages_out, budget, n_sink, n_recent)
 
 
+@functools.lru_cache(_PLANS)
+def _plan_evict(k, v, weights, seqlens_k, block_table, k_out, v_out, out_table, weights_out, seqlens_out, kept, budget, n_sink, n_recent):
+    k, v, weights, seqlens_k, block_table, k_out, v_out, out_table, weights_out, seqlens_out, kept = _sigs(
+        k, v, weights, seqlens_k, block_table, k_out, v_out, out_table, weights_out, seqlens_out, kept)
+    if (k_out is None) != (v_out is None):
+        raise ValueError("k_out and v_out must be given together")
+    _half(k, v, k_out, v_out)
+    if k.shape != v.shape:
+        raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} do not fit together")
+    b, hk = seqlens_k.shape[0] if len(seqlens_k.shape) == 1 else -1, k.shape[2]
+    if k_out is None:
+        if out_table is not None:
+            raise ValueError("out_table without k_out")
+        k_out, v_out, out_table = k, v, block_table
+    elif k_out.shape != v_out.shape or k_out.shape[2:] != k.shape[2:]:
+        raise ValueError(f"k_out {tuple(k_out.shape)} and v_out {tuple(v_out.shape)} do not fit k {tuple(k.shape)}")
+    if _overlaps(k_out) or _overlaps(v_out):
+        raise ValueError("rows cannot be moved to a broadcast view")
+    max_pages, cap = _table(block_table, k, b, "block_table")
+    max_pages_out, cap_out = _table(out_table, k_out, b, "out_table")
+    for t, dtype, shape, what in ((seqlens_k, torch.int32, (b,), "seqlens_k"), (seqlens_out, torch.int32, (b,), "seqlens_out"),
+                                  (kept, torch.int32, (b, hk, budget), "kept"), (weights, torch.float32, (b, hk, cap), "weights"),
+                                  (weights_out, torch.float32, (b, hk, cap_out), "weights_out")):
+        _like(t, dtype, shape, what)
+        _dense(t, what)
+    _on(k.device, v, weights, seqlens_k, block_table, k_out, v_out, out_table, weights_out, seqlens_out, kept)
+    return _plan("evict", k.dtype, _evict_blob(k, v, k_out, v_out, b, max_pages, max_pages_out, budget, n_sink, n_recent)) + (cap_out,)
+
+
+@_on_stream
 def flash_attn_evict(k, v, weights, seqlens_k, budget, n_sink=0, n_recent=0, block_table=None, k_out=None, v_out=None, out_table=None,
-                     weights_out=None, seqlens_out=None, kept=None, stream=None):
+                     weights_out=None, seqlens_out=None, kept=None):
     """Cuts every (sequence, key/value head) of a cache to `budget` rows: the first n_sink, the last n_recent
     and, of those between, the ones of greatest weight (equal weights: the lower row; NaN below everything)
     stay and move to the front in their order.  k, v: pages with block_table, or dense [b, s, h_k, d];
@@ -496,46 +653,18 @@ def flash_attn_evict(k, v, weights, seqlens_k, budget, n_sink=0, n_recent=0, blo
     at most `budget` rows keeps them all; a negative length stays.  Rows, weights behind the last kept
     one and rows of absent pages are left as they were.
     -> (kept int32 [b, h_k, budget]: the row each came from, -1 behind the last; weights_out; seqlens_out)."""
-    _half(k, v, k_out, v_out)
-    if k.shape != v.shape:
-        raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} do not fit together")
-    if (k_out is None) != (v_out is None):
-        raise ValueError("k_out and v_out must be given together")
-    b, hk = seqlens_k.shape[0] if seqlens_k.dim() == 1 else -1, k.shape[2]
+    plan = _plan_evict(_sig(k), _sig(v), _sig(weights), _sig(seqlens_k), _sig(block_table), _sig(k_out), _sig(v_out), _sig(out_table),
+                       _sig(weights_out), _sig(seqlens_out), _sig(kept), budget, n_sink, n_recent)
     in_place = k_out is None
+    b, hk = seqlens_k.shape[0], k.shape[2]
     if in_place:
-        if out_table is not None:
-            raise ValueError("out_table without k_out")
         k_out, v_out, out_table = k, v, block_table
-    elif k_out.shape != v_out.shape or k_out.shape[2:] != k.shape[2:]:
-        raise ValueError(f"k_out {tuple(k_out.shape)} and v_out {tuple(v_out.shape)} do not fit k {tuple(k.shape)}")
-    if _overlaps(k_out) or _overlaps(v_out):
-        raise ValueError("rows cannot be moved to a broadcast view")
-    caps = []
-    for t, pages, what in ((block_table, k, "block_table"), (out_table, k_out, "out_table")):
-        if t is not None and (t.dim() != 2 or t.shape[1] == 0):
-            raise ValueError(f"{what} must be [b, max_pages] with at least one page")
-        if t is None and pages.shape[0] != b:
-            raise ValueError(f"{b} sequences, but a dense cache of {pages.shape[0]}")
-        if t is not None:
-            _like(t, torch.int32, (b, t.shape[1]), what)
-        _dense(t, what)
-        caps.append((t.shape[1] if t is not None else 1) * pages.shape[1])
     if weights_out is None:
-        weights_out = weights if in_place else torch.zeros((b, hk, caps[1]), dtype=torch.float32, device=k.device)
+        weights_out = weights if in_place else torch.zeros((b, hk, plan[4]), dtype=torch.float32, device=k.device)
     if seqlens_out is None:
         seqlens_out = seqlens_k if in_place else torch.empty_like(seqlens_k)
     if kept is None:
-        kept = torch.empty((b, hk, max(budget, 0)), dtype=torch.int32, device=k.device)
-    _like(seqlens_k, torch.int32, (b,), "seqlens_k")
-    _like(seqlens_out, torch.int32, (b,), "seqlens_out")
-    _like(kept, torch.int32, (b, hk, budget), "kept")
-    _like(weights, torch.float32, (b, hk, caps[0]), "weights")
-    _like(weights_out, torch.float32, (b, hk, caps[1]), "weights_out")
-    for t, what in ((weights, "weights"), (weights_out, "weights_out"), (seqlens_k, "seqlens_k"), (seqlens_out, "seqlens_out"), (kept, "kept")):
-        _dense(t, what)
-    _on(k.device, v, weights, seqlens_k, block_table, k_out, v_out, out_table, weights_out, seqlens_out, kept)
-    blob = pack_flash_evict_args(k, v, k_out, v_out, b, block_table.shape[1] if block_table is not None else 0,
-                                 out_table.shape[1] if out_table is not None else 0, budget, n_sink, n_recent)
-    _call_checked("evict", [k, v, weights, seqlens_k, block_table, k_out, v_out, out_table, weights_out, seqlens_out, kept], blob, k.device, k.dtype, None, stream)
+        kept = torch.empty((b, hk, budget), dtype=torch.int32, device=k.device)
+    _launch(plan[:4], _pack11(k.data_ptr(), v.data_ptr(), weights.data_ptr(), seqlens_k.data_ptr(), _ptr(block_table), k_out.data_ptr(), v_out.data_ptr(),
+                              _ptr(out_table), weights_out.data_ptr(), seqlens_out.data_ptr(), kept.data_ptr()), k, None)
     return kept, weights_out, seqlens_out

@@ -234,6 +234,7 @@ using std::min;
 #define __builtin_amdgcn_readfirstlane(...) ::fa_emu::readfirstlane_any(__VA_ARGS__)
 #define __builtin_amdgcn_permlane32_swap(...) ::fa_emu::permlane32_swap(__VA_ARGS__)
 #define __builtin_amdgcn_ds_bpermute(...) ::fa_emu::ds_bpermute(__VA_ARGS__)
+#define __builtin_amdgcn_readlane(v, lane) ::fa_emu::ds_bpermute((lane) * 4, (v))
 #define __builtin_amdgcn_exp2f(...) ::exp2f(__VA_ARGS__)
 #define __builtin_amdgcn_logf(...) ::log2f(__VA_ARGS__)
 #define __builtin_amdgcn_fdot2(...) ::fa_emu::fdot2(__VA_ARGS__)
