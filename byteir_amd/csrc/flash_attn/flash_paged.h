@@ -14,18 +14,18 @@ struct Pages {
   int shift;
   int64_t k_ps, k_rs, k_hs, v_ps, v_rs, v_hs;  // page, row and head strides (elements)
   FA_HD int capacity() const { return max_pages ? max_pages * page : page; }
-  // the table's page number for a key, and the key's row there ...
-  __device__ __forceinline__ int number(int bi, int key, int &row) const {
-    if (!max_pages) { row = key; return bi; }
+  // the place of a key in the sequence's row of the table, and the key's row on that page
+  __device__ __forceinline__ int index(int key, int &row) const {
     const int at = (int)(((uint64_t)(uint32_t)key * mul) >> shift);
     row = key - at * page;
-    return table[(int64_t)bi * max_pages + at];
+    return at;
   }
-  // ... which names a page when it lies inside the pool
+  // a number names a page when it lies inside the pool
   __device__ __forceinline__ bool present(int pg) const { return (unsigned)pg < (unsigned)num_pages; }
-  // both: the page, or -1 when it is absent
+  // page of a key and its row there; -1: the page is absent
   __device__ __forceinline__ int locate(int bi, int key, int &row) const {
-    const int pg = number(bi, key, row);
+    if (!max_pages) { row = key; return bi; }
+    const int pg = table[(int64_t)bi * max_pages + index(key, row)];
     return present(pg) ? pg : -1;
   }
 };

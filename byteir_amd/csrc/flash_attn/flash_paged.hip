@@ -35,8 +35,10 @@ __global__ void __launch_bounds__(kWaves * 64, D <= 128 ? 2 : 1) paged_kernel(co
   constexpr int RPP = 64 / CPR;      // rows per pass of a wave
   constexpr int NPV = kUnit / RPP;   // passes per unit
   constexpr int kWaveLds = kUnit * (KS + VS) * (int)sizeof(T);  // a wave's K and V tile, reused for the join
-  static_assert(kWaveLds >= (D * 32 + 64) * 4, "join buffers must fit the tiles");
+  constexpr int OS = D + 4;  // row stride of a wave's O when the waves join
+  static_assert(kWaveLds >= 32 * OS * 4, "a wave's O must fit its tiles");
   __shared__ __attribute__((aligned(16))) unsigned char lds[kWaves][kWaveLds];
+  __shared__ float m_s[kWaves][32], l_s[kWaves][32];
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);  // a scalar: units, masks and branches on them are the wave's
@@ -84,13 +86,19 @@ __global__ void __launch_bounds__(kWaves * 64, D <= 128 ? 2 : 1) paged_kernel(co
   const T *kng = p.fuse_append ? static_cast<const T *>(p.k_new) + bi * p.kn_bs + hk * p.kn_hs : nullptr;
   const T *vng = p.fuse_append ? static_cast<const T *>(p.v_new) + bi * p.vn_bs + hk * p.vn_hs : nullptr;
   // Where row l % 32 of a unit lies, in lane l: its page number and its row there (-1: nobody sees
-  // the row); requested a unit ahead of the loads that need it.  The number is not looked at
-  // here: a test would wait for it and with it for every load in flight.
-  int pg_next = 0, row_next = -1;
+  // the row); requested a unit ahead of the loads that need it.  The request is unconditional
+  // (some entry of the table, or any word when there is none) and its result is not looked at
+  // here: a test, or a choice between it and something else, would wait for it and with it for
+  // every load in flight.
+  const int *table = p.pages.max_pages ? p.pages.table + (int64_t)bi * p.pages.max_pages : p.seqlens;
+  int number_next = 0, row_next = -1;
   auto locate = [&](int j) {
     const int key = idx::sink_tile(st, j) * kUnit + r32;
-    row_next = -1;
-    if (key < st.hi && (key >= st.lo || key < st.sink)) pg_next = p.pages.number(bi, key, row_next);
+    const bool seen = key < st.hi && (key >= st.lo || key < st.sink);
+    int at = 0, row = key;
+    if (p.pages.max_pages) at = p.pages.index(seen ? key : 0, row);
+    number_next = table[at];
+    row_next = seen ? row : -1;
   };
   auto from_lane = [&](int64_t v, int src) {  // lane src's value
     const int lo = __builtin_amdgcn_ds_bpermute(src * 4, (int)v), hi = __builtin_amdgcn_ds_bpermute(src * 4, (int)(v >> 32));
@@ -99,12 +107,25 @@ __global__ void __launch_bounds__(kWaves * 64, D <= 128 ? 2 : 1) paged_kernel(co
   // The rows of one pass lie on one page when the page size is a multiple of their number: their
   // address is then a scalar plus an offset that every pass shares, which costs the vector ALU
   // and the registers nothing.
-  const bool scalar_rows = p.pages.page % RPP == 0 && p.d == D && (uint64_t)p.pages.k_rs < (1 << 26) && (uint64_t)p.pages.v_rs < (1 << 26);
-  const uint32_t k_in = (uint32_t)(v_r * (uint32_t)p.pages.k_rs + v_c * 8), v_in = (uint32_t)(v_r * (uint32_t)p.pages.v_rs + v_c * 8);
-  auto load_unit = [&](int j) -> uint32_t {  // unit j, located, into the staging registers -> which of its rows exist
-    const int kv0 = idx::sink_tile(st, j) * kUnit;
+  const bool scalar_rows = p.pages.page % RPP == 0 && (uint64_t)p.pages.k_rs < (1 << 26) && (uint64_t)p.pages.v_rs < (1 << 26);
+  const bool col_in = v_c * 8 < p.d;            // columns from head_dim up to D are zeros in the tiles
+  const int v_col = col_in ? v_c * 8 : 0;       // their lanes load a column that exists and store nothing
+  const uint32_t k_in = (uint32_t)(v_r * (uint32_t)p.pages.k_rs + v_col), v_in = (uint32_t)(v_r * (uint32_t)p.pages.v_rs + v_col);
+  // Unit j, located, into the staging registers, when all its 32 rows are to be read from the
+  // cache; -> which of its rows exist.  A unit with rows that are not (the ends of a sequence or
+  // window, absent pages, new rows) is read by store_unit instead: keeping it in flight as well would
+  // cost the registers that the LDS reads of the loop need to run ahead of the MFMAs.
+  int pg_cur = 0, row_cur = -1;
+  bool staged = false;
+  auto load_unit = [&](int j) -> uint32_t {
+    const int pg_next = p.pages.max_pages ? number_next : bi;
     const uint32_t there = (uint32_t)__builtin_amdgcn_ballot_w64(row_next >= 0 && p.pages.present(pg_next));
-    if (there == 0xffffffffu && kv0 + kUnit <= new0 && scalar_rows) {  // a whole unit of the cache
+    pg_cur = pg_next;
+    row_cur = row_next;
+    int vr = v_r;
+    FA_PIN(vr);  // what the uncommon paths derive from it is computed there, not kept in registers over the loop
+    staged = there == 0xffffffffu && idx::sink_tile(st, j) * kUnit + kUnit <= new0;
+    if (staged && scalar_rows) {
 #pragma unroll
       for (int s = 0; s < NPV; ++s) {
         const int64_t pg = __builtin_amdgcn_readlane(pg_next, s * RPP), row = __builtin_amdgcn_readlane(row_next, s * RPP);
@@ -113,35 +134,65 @@ __global__ void __launch_bounds__(kWaves * 64, D <= 128 ? 2 : 1) paged_kernel(co
         kn[s] = uint4{a.x, a.y, a.z, a.w};
         vn[s] = uint4{b.x, b.y, b.z, b.w};
       }
-      return there;
-    }
-    const int64_t k_lane = pg_next * p.pages.k_ps + row_next * p.pages.k_rs, v_lane = pg_next * p.pages.v_ps + row_next * p.pages.v_rs;
+    } else if (staged) {
+      const int64_t k_lane = pg_next * p.pages.k_ps + row_next * p.pages.k_rs, v_lane = pg_next * p.pages.v_ps + row_next * p.pages.v_rs;
 #pragma unroll
-    for (int s = 0; s < NPV; ++s) {
-      const int r = s * RPP + v_r, key = kv0 + r;
-      const int64_t ko = from_lane(k_lane, r), vo = from_lane(v_lane, r);
-      kn[s] = uint4{0, 0, 0, 0};  // a row that nobody sees: 0 * finite stays finite in P V
-      vn[s] = uint4{0, 0, 0, 0};
-      if (((there >> r) & 1u) && v_c * 8 < p.d) {  // columns from head_dim up to D stay zero
-        const bool fresh = key >= new0;
-        kn[s] = *reinterpret_cast<const uint4 *>((fresh ? kng + (int64_t)(key - new0) * p.kn_rs : kg + ko) + v_c * 8);
-        vn[s] = *reinterpret_cast<const uint4 *>((fresh ? vng + (int64_t)(key - new0) * p.vn_rs : vg + vo) + v_c * 8);
-        if (fresh) {
-          *reinterpret_cast<uint4 *>(const_cast<T *>(kg) + ko + v_c * 8) = kn[s];
-          *reinterpret_cast<uint4 *>(const_cast<T *>(vg) + vo + v_c * 8) = vn[s];
-        }
+      for (int s = 0; s < NPV; ++s) {
+        const int64_t ko = from_lane(k_lane, s * RPP + vr), vo = from_lane(v_lane, s * RPP + vr);
+        const u32x4 a = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(kg + ko + v_col));
+        const u32x4 b = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(vg + vo + v_col));
+        kn[s] = uint4{a.x, a.y, a.z, a.w};
+        vn[s] = uint4{b.x, b.y, b.z, b.w};
       }
     }
     return there;
   };
-  auto store_unit = [&]() {
+  auto store_unit = [&](int j, uint32_t there) {  // unit j into the wave's tiles
+    if (!staged) {
+      const int kv0 = idx::sink_tile(st, j) * kUnit;
+      int vr = v_r;
+      FA_PIN(vr);
+      const int64_t k_lane = pg_cur * p.pages.k_ps + row_cur * p.pages.k_rs, v_lane = pg_cur * p.pages.v_ps + row_cur * p.pages.v_rs;
 #pragma unroll
-    for (int s = 0; s < NPV; ++s) {
-      *reinterpret_cast<uint4 *>(&Kt[(s * RPP + v_r) * KS + v_c * 8]) = kn[s];
-      *reinterpret_cast<uint4 *>(&Vt[(s * RPP + v_r) * VS + v_c * 8]) = vn[s];
+      for (int s = 0; s < NPV; ++s) {
+        const int r = s * RPP + vr, key = kv0 + r;
+        const int64_t ko = from_lane(k_lane, r), vo = from_lane(v_lane, r);
+        const bool fresh = key >= new0;
+        kn[s] = uint4{0, 0, 0, 0};  // a row that nobody sees: 0 * finite stays finite in P V
+        vn[s] = uint4{0, 0, 0, 0};
+        if (((there >> r) & 1u) & col_in) {
+          kn[s] = *reinterpret_cast<const uint4 *>((fresh ? kng + (int64_t)(key - new0) * p.kn_rs : kg + ko) + v_col);
+          vn[s] = *reinterpret_cast<const uint4 *>((fresh ? vng + (int64_t)(key - new0) * p.vn_rs : vg + vo) + v_col);
+        }
+      }
+      if (kv0 + kUnit > new0) {
+#pragma unroll
+        for (int s = 0; s < NPV; ++s) {
+          const int r = s * RPP + vr;
+          const int64_t ko = from_lane(k_lane, r), vo = from_lane(v_lane, r);
+          if (((there >> r) & 1u) && col_in && kv0 + r >= new0) {
+            *reinterpret_cast<uint4 *>(const_cast<T *>(kg) + ko + v_col) = kn[s];
+            *reinterpret_cast<uint4 *>(const_cast<T *>(vg) + vo + v_col) = vn[s];
+          }
+        }
+      }
+    }
+    if (col_in) {
+#pragma unroll
+      for (int s = 0; s < NPV; ++s) {
+        *reinterpret_cast<uint4 *>(&Kt[(s * RPP + v_r) * KS + v_c * 8]) = kn[s];
+        *reinterpret_cast<uint4 *>(&Vt[(s * RPP + v_r) * VS + v_c * 8]) = vn[s];
+      }
     }
     FA_WAVE_SYNC();  // the wave's own tile: written by all its lanes, read across lanes, no workgroup barrier
   };
+  if (p.d != D && !col_in) {
+#pragma unroll
+    for (int s = 0; s < NPV; ++s) {
+      *reinterpret_cast<uint4 *>(&Kt[(s * RPP + v_r) * KS + v_c * 8]) = uint4{0, 0, 0, 0};
+      *reinterpret_cast<uint4 *>(&Vt[(s * RPP + v_r) * VS + v_c * 8]) = uint4{0, 0, 0, 0};
+    }
+  }
 
   float16v o_acc[D / 32];
 #pragma unroll
@@ -156,8 +207,8 @@ __global__ void __launch_bounds__(kWaves * 64, D <= 128 ? 2 : 1) paged_kernel(co
   if (u0 + wave < u1) {
     locate(u0 + wave);
     there = load_unit(u0 + wave);
-    if (u0 + wave + kWaves < u1) locate(u0 + wave + kWaves);
-    store_unit();
+    locate(min(u0 + wave + kWaves, u1 - 1));
+    store_unit(u0 + wave, there);
   }
   // The Q fragments are consumed here: the wait for their loads would otherwise stand before the first
   // MFMA of every unit and drain the loads of the next one too.
@@ -168,7 +219,7 @@ __global__ void __launch_bounds__(kWaves * 64, D <= 128 ? 2 : 1) paged_kernel(co
     uint32_t there_next = 0;
     if (has_next) {
       there_next = load_unit(j + kWaves);
-      if (j + 2 * kWaves < u1) locate(j + 2 * kWaves);
+      locate(min(j + 2 * kWaves, u1 - 1));
     }
     float16v s = float16v{0};
 #pragma unroll
@@ -179,7 +230,8 @@ __global__ void __launch_bounds__(kWaves * 64, D <= 128 ? 2 : 1) paged_kernel(co
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const int r = (i >> 2) * 8 + g * 4 + (i & 3), kv = kv0 + r;
-        if (kv >= hi_lim || (kv < lo_lim && kv >= p.n_sink) || !((there >> r) & 1u)) s[i] = -INFINITY;
+        const bool hidden = (kv >= hi_lim) | ((kv < lo_lim) & (kv >= p.n_sink)) | !((there >> r) & 1u);
+        s[i] = hidden ? -INFINITY : s[i];
       }
     }
     if constexpr (Scores) {
@@ -225,33 +277,34 @@ __global__ void __launch_bounds__(kWaves * 64, D <= 128 ? 2 : 1) paged_kernel(co
       for (int db = 0; db < D / 32; ++db)
         o_acc[db] = Traits<T>::mfma(lds_read_operand_tr<T>(Vt, VS, w * 16, db * 32), pb, o_acc[db]);
     }
-    if (has_next) store_unit();  // after every read of unit j in program order
+    if (has_next) store_unit(j + kWaves, there_next);  // after every read of unit j in program order
     there = there_next;
   }
 
   // ---- the four waves' partials joined through LDS (each wave writes into its own region) ----
   const float l_wave = l_run + partner32(l_run);
-  float *Ow = reinterpret_cast<float *>(lds[wave]);  // [D][32]
-  float *MLw = Ow + D * 32;                          // [2][32]
+  float *Ow = reinterpret_cast<float *>(lds[wave]);  // [32 columns][OS]
 #pragma unroll
   for (int db = 0; db < D / 32; ++db)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) Ow[(db * 32 + (i >> 2) * 8 + g * 4 + (i & 3)) * 32 + r32] = o_acc[db][i];
-  if (g == 0) { MLw[r32] = m_run; MLw[32 + r32] = l_wave; }
+    for (int i4 = 0; i4 < 4; ++i4)
+      *reinterpret_cast<float4 *>(&Ow[r32 * OS + db * 32 + i4 * 8 + g * 4]) =
+          float4{o_acc[db][i4 * 4], o_acc[db][i4 * 4 + 1], o_acc[db][i4 * 4 + 2], o_acc[db][i4 * 4 + 3]};
+  if (g == 0) { m_s[wave][r32] = m_run; l_s[wave][r32] = l_wave; }
   __syncthreads();
 
   const int on = tid & 31, slice = tid >> 5;  // eight slices of D / 8 output elements per column
   float mw[kWaves], wgt[kWaves], m_all = -INFINITY, l_all = 0.f;
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) {
-    mw[w] = reinterpret_cast<const float *>(lds[w])[D * 32 + on];
+    mw[w] = m_s[w][on];
     m_all = fmaxf(m_all, mw[w]);
   }
   const float m_ref = m_all == -INFINITY ? 0.f : m_all;
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) {
     wgt[w] = exp2_fast((mw[w] - m_ref) * c);  // 0 for a wave that saw no key
-    l_all += wgt[w] * reinterpret_cast<const float *>(lds[w])[D * 32 + 32 + on];
+    l_all += wgt[w] * l_s[w][on];
   }
   const int cn = ct * 32 + on;
   if (cn >= n_cols) return;
@@ -264,12 +317,11 @@ __global__ void __launch_bounds__(kWaves * 64, D <= 128 ? 2 : 1) paged_kernel(co
 #pragma unroll
   for (int x = 0; x < D / 8; x += 4) {
     const int dcol = slice * (D / 8) + x;
-    float acc[4];
+    float acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int y = 0; y < 4; ++y) {
-      acc[y] = 0.f;
-#pragma unroll
-      for (int w = 0; w < kWaves; ++w) acc[y] += wgt[w] * reinterpret_cast<const float *>(lds[w])[(dcol + y) * 32 + on];
+    for (int w = 0; w < kWaves; ++w) {
+      const float4 t = *reinterpret_cast<const float4 *>(&reinterpret_cast<const float *>(lds[w])[on * OS + dcol]);
+      acc[0] += wgt[w] * t.x; acc[1] += wgt[w] * t.y; acc[2] += wgt[w] * t.z; acc[3] += wgt[w] * t.w;
     }
     typedef T vec4 __attribute__((ext_vector_type(4)));
     if (!final_pass) *reinterpret_cast<float4 *>(p.o_part + prow * D + dcol) = float4{acc[0], acc[1], acc[2], acc[3]};
@@ -429,10 +481,11 @@ hipError_t launch_paged(PagedParams &p, int dtype, hipStream_t stream) {
     units = std::min<int64_t>(units, (std::min(p.n_sink, cap) + kUnit - 1) / kUnit + ((int64_t)p.wl + p.sq + kUnit) / kUnit + 2);
   p.max_units = (int)std::max<int64_t>(units, 1);
   const int64_t base = (int64_t)p.b * p.h_k * p.n_ct;
-  // Splits: enough workgroups that unequal sequences even out (8 for every CU, two of them at a time),
-  // of at least 512 keys each when there are many and 128 (a unit a wave) when there are few
-  const int64_t want = std::max<int64_t>(1, 2048 / base);
-  p.min_units = (int)std::min<int64_t>(16, std::max<int64_t>(kWaves, p.max_units / want));
+  // Splits: one round of workgroups (two for every CU) when the sequences are few, of 128 keys (a unit
+  // a wave) at least; 2048 keys each when they are many, so that unequal lengths even out.  Units
+  // per split 16 / 32 / 64 / 128, kernel time: 64 x 8192 keys, 8 heads, D = 128: 368 / 351 / 346 /
+  // 340 us, 1000..8191 keys: 231 / 212 / 211 / 238 with the join; 8 x 8192: 55 / 52 / 56 / 87.
+  p.min_units = (int)std::min<int64_t>(64, std::max<int64_t>(kWaves, (p.max_units * base + 511) / 512));
   p.n_splits = p.max_units <= 2 * kWaves ? 1 : (int)std::min<int64_t>(64, (p.max_units + p.min_units - 1) / p.min_units);
   // the attention kernel appends when one workgroup's tile covers all columns and its window reaches the first new row
   p.fuse_append = p.n_new > 0 && p.n_ct == 1 && (p.wl < 0 || p.n_new <= (int64_t)p.sq + p.wl);
