@@ -214,8 +214,12 @@ __global__ void __launch_bounds__(256, DR <= 128 ? 2 : 1) fwd_anyd_kernel(const 
   row_limits_sk(p, sk, m0 + kRows - 1, t1, b_hi);
   idx::SinkTiles st{};
   if constexpr (Sink) st = idx::sink_tile_range(p.sq, sk, p.wl, p.wr, p.n_sink, m0, kRows, kTile);
-  const int n_min = Sink ? 0 : b_lo / kTile;
-  const int n_max = Sink ? st.n : b_hi > 0 ? (b_hi + kTile - 1) / kTile : 0;
+  int n_min = Sink ? 0 : b_lo / kTile;
+  int n_max = Sink ? st.n : b_hi > 0 ? (b_hi + kTile - 1) / kTile : 0;
+  if (Sink && p.n_splits > 1) {  // the list of tiles shared out over workgroups
+    n_min = blockIdx.y * p.split_tiles;
+    n_max = min(n_max, n_min + p.split_tiles);
+  }
   auto tile_kv0 = [&](int t) { return (Sink ? idx::sink_tile(st, t) : t) * kTile; };  // first key of the t-th tile
 
   const T *qg = static_cast<const T *>(p.q) + bi * p.q_bs + (int64_t)qrow * p.q_rs + hi * p.q_hs;
@@ -342,6 +346,16 @@ __global__ void __launch_bounds__(256, DR <= 128 ? 2 : 1) fwd_anyd_kernel(const 
   const bool empty = l_tot == 0.f || l_tot != l_tot;
   float inv = empty ? 1.f : 1.f / l_tot;
   if constexpr (Drop) inv *= p.rp_keep;
+  if (Sink && p.n_splits > 1) {  // unnormalised partial, relative to this split's maximum
+    if (qrow < p.sq) {
+      constexpr int W = DR <= 32 ? 32 : DR <= 64 ? 64 : DR <= 128 ? 128 : 256;
+      const int64_t prow = (((int64_t)blockIdx.y * p.b + bi) * p.h + hi) * p.sq + qrow;
+#pragma unroll
+      for (int db = 0; db < DR / 32; ++db) store_acc<float>(p.o_part + prow * W, o_acc[db], db, g, 1.f, p.d);
+      if (g == 0) { p.ml_part[prow * 2] = m_run; p.ml_part[prow * 2 + 1] = l_tot; }
+    }
+    return;
+  }
   if (qrow < p.sq) {
     T *og = static_cast<T *>(p.o_w) + bi * p.o_bs + (int64_t)qrow * p.o_rs + hi * p.o_hs;
 #pragma unroll
@@ -686,11 +700,45 @@ __global__ void __launch_bounds__(256, (DR <= 96 || (DR == 128 && !Drop)) ? 2 : 
   }
 }
 
+// With sinks the list of tiles is split over workgroups when the grid does not fill the chip (two
+// workgroups for every CU up to 128 columns, at least four tiles a split) and the list is long for the
+// number of rows that a join would have to go through.
 template <typename T, int DR>
-hipError_t fwd_anyd_d(const Params &p, hipStream_t stream) {
+hipError_t fwd_anyd_sink(Params &p, hipStream_t stream) {
+  const int n_wg = p.n_mblocks * p.b * p.h, n_tiles = sink_tiles_bound(p, kRows, kTile);
+  const int64_t n_rows = (int64_t)p.b * p.h * p.sq;
+  const int n_splits = n_rows > 512 * (int64_t)n_tiles ? 1 : pick_splits(n_wg, n_tiles, DR <= 128 ? 512 : 256, 4);
+  const int width = DR <= 32 ? 32 : DR <= 64 ? 64 : DR <= 128 ? 128 : 256;
+  const size_t rows = (size_t)p.b * p.h * p.sq, need = n_splits > 1 ? n_splits * rows * (width + 2) * sizeof(float) : 0;
+  if (p.ws_query) { *p.ws_query = need; return hipSuccess; }
+  void *ws = nullptr, *owned = nullptr;
+  p.n_splits = 1;
+  if (need) {
+    if (p.ws && (reinterpret_cast<uintptr_t>(p.ws) & 15) == 0 && p.ws_bytes >= need) ws = p.ws;
+    else if (hipMallocAsync(&owned, need, stream) == hipSuccess) ws = owned;
+    else { (void)hipGetLastError(); owned = nullptr; }  // no scratch: one split
+  }
+  if (ws) {
+    p.n_splits = n_splits;
+    p.split_tiles = (n_tiles + n_splits - 1) / n_splits;
+    p.o_part = static_cast<float *>(ws);
+    p.ml_part = p.o_part + (size_t)n_splits * rows * width;
+  }
+  FA_LAUNCH((fwd_anyd_kernel<T, DR, false, true>), dim3((unsigned)n_wg, (unsigned)p.n_splits), dim3(256), stream, p);
+  hipError_t e = hipGetLastError();
+  if (ws && e == hipSuccess) e = launch_sink_join(p, width, std::is_same<T, _Float16>::value ? 1 : 2, stream);
+  if (owned) {
+    const hipError_t f = hipFreeAsync(owned, stream);
+    if (e == hipSuccess) e = f;
+  }
+  return e;
+}
+
+template <typename T, int DR>
+hipError_t fwd_anyd_d(Params &p, hipStream_t stream) {
+  if (p.sink) return fwd_anyd_sink<T, DR>(p, stream);
   const dim3 grid((unsigned)(p.n_mblocks * p.b * p.h)), block(256);
-  if (p.sink) FA_LAUNCH((fwd_anyd_kernel<T, DR, false, true>), grid, block, stream, p);
-  else if (p.drop) FA_LAUNCH((fwd_anyd_kernel<T, DR, true>), grid, block, stream, p);
+  if (p.drop) FA_LAUNCH((fwd_anyd_kernel<T, DR, true>), grid, block, stream, p);
   else FA_LAUNCH((fwd_anyd_kernel<T, DR, false>), grid, block, stream, p);
   return hipGetLastError();
 }
@@ -724,7 +772,7 @@ hipError_t bwd_anyd_d(const Params &p, hipStream_t stream) {
 }
 
 template <typename T>
-hipError_t fwd_anyd_t(const Params &p, hipStream_t stream) {
+hipError_t fwd_anyd_t(Params &p, hipStream_t stream) {
   if (p.d <= 32) return fwd_anyd_d<T, 32>(p, stream);
   if (p.d <= 64) return fwd_anyd_d<T, 64>(p, stream);
   if (p.d <= 96) return fwd_anyd_d<T, 96>(p, stream);
@@ -750,7 +798,7 @@ hipError_t bwd_anyd_t(const Params &p, hipStream_t stream) {
 hipError_t launch_fwd_anyd(Params &p, int dtype, hipStream_t stream) {
   if (p.d <= 0 || p.d > 256 || p.d % 8 != 0) return hipErrorInvalidValue;
   p.n_mblocks = (p.sq + kRows - 1) / kRows;
-  if (p.n_mblocks == 0 || p.ws_query) return hipSuccess;  // this path takes no scratch
+  if (p.n_mblocks == 0 || (p.ws_query && !p.sink)) return hipSuccess;  // without sinks this path takes no scratch
   return dtype == 1 ? fwd_anyd_t<_Float16>(p, stream) : fwd_anyd_t<__bf16>(p, stream);
 }
 

@@ -13,6 +13,8 @@
 #pragma once
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+#include <cmath>
 #include <cstdint>
 #include <type_traits>
 
@@ -299,10 +301,46 @@ inline void apply_group_split(Params &pk, const Params &p, const GroupSplit &s, 
 }
 hipError_t launch_group_sum(const Params &p, const GroupSplit &s, int row, int dtype, hipStream_t stream);
 
+// attention with sinks of a few query rows: the paged kernel over the dense keys (flash_paged.hip)
+bool sink_few_rows(const Params &p);
+// joins p.n_splits partials with rows of `width` floats into p.o_w and p.lse
+hipError_t launch_sink_join(const Params &p, int width, int dtype, hipStream_t stream);
+hipError_t launch_sink_few_rows(const Params &p, int dtype, hipStream_t stream);
+// most key tiles of `bn` rows that a block of `bm` query rows of a flash_attn_sink_fwd call visits
+inline int sink_tiles_bound(const Params &p, int bm, int bn) {
+  const int all = (p.sk + bn - 1) / bn;
+  if (p.wl < 0 || p.wr < 0) return all;
+  const int64_t most = (int64_t)(std::min(p.n_sink, p.sk) + bn - 1) / bn + ((int64_t)p.wl + p.wr + bm) / bn + 2;
+  return (int)std::min<int64_t>(all, most);
+}
+
 // dK / dV of the sink keys (flash_sink.hip): replaces the rows that the windowed kernel wrote;
 // sink_dkdv_bytes is the scratch it takes
 size_t sink_dkdv_bytes(const Params &p);
 hipError_t launch_sink_dkdv(const Params &p, int dtype, void *ws, size_t ws_bytes, hipStream_t stream);
+
+// Number of key-axis splits for `n_wg` workgroups over `n_tiles` key tiles on 256 CUs: as the
+// reference's num_splits_heuristic (flash_api.cu:118-160) -- one split when the chip is already
+// 80 % full; otherwise the smallest count whose last round of workgroups is at least 85 % as
+// full as the best count's -- with at most 32 splits of at least eight tiles.
+// (slots, min_tiles: other workgroup slots on the chip, other least tiles of a split)
+inline int pick_splits(int n_wg, int n_tiles, int slots = 256, int min_tiles = 8) {
+  const int kCUs = slots;
+  if (n_wg >= 0.8f * kCUs) return 1;
+  const int max_splits = std::min(32, n_tiles / min_tiles);
+  auto tiles_per = [&](int s) { return (n_tiles + s - 1) / s; };
+  auto eligible = [&](int s) { return s == 1 || tiles_per(s) != tiles_per(s - 1); };
+  auto eff = [&](int s) {
+    const float waves = float(n_wg * s) / kCUs;
+    return waves / std::ceil(waves);
+  };
+  float best = 0.f;
+  for (int s = 1; s <= max_splits; ++s)
+    if (eligible(s)) best = std::max(best, eff(s));
+  for (int s = 1; s <= max_splits; ++s)
+    if (eligible(s) && eff(s) >= 0.85f * best) return s;
+  return 1;
+}
 
 // A few query rows against a long key sequence (flash_decode.hip): all query heads of a
 // key/value head times all query rows must fit the 32 columns of one score tile.

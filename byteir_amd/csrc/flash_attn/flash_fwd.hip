@@ -38,7 +38,9 @@ constexpr float kRescaleSlack = 8.0f;
 // VarK: the number of keys is read per batch (key/value cache calls): seqlens_k[b] + seqlen_knew
 // Sink: keys [0, p.n_sink) stay visible outside the window (idx::sink_tile_range): their tiles come
 // first, then the window's, as one list of tiles walked by the same loop; a tile row that none
-// of the workgroup's query rows can see is read as zeros, whatever it holds
+// of the workgroup's query rows can see is read as zeros, whatever it holds.  Here D may exceed
+// head_dim: the columns behind it are zeros on the way in and not written (a head_dim of 80 at
+// D = 128 takes two thirds of the time of the generic kernel at 96 columns).
 template <typename T, int D, int QB, int NW, bool VarK, bool Sink = false>
 __global__ void __launch_bounds__(NW * 64, NW * QB >= 16 ? 2 : (QB == 2 ? 1 : 2)) flash_fwd_kernel(const Params p) {
   constexpr int kThreads = NW * 64;
@@ -107,7 +109,7 @@ __global__ void __launch_bounds__(NW * 64, NW * QB >= 16 ? 2 : (QB == 2 ? 1 : 2)
     const T *qg = static_cast<const T *>(p.q) + bi * p.q_bs + (int64_t)qrow[qb] * p.q_rs + hi * p.q_hs;
 #pragma unroll
     for (int ks = 0; ks < D / 16; ++ks) {
-      if (qrow[qb] < p.sq) qf[qb][ks] = *reinterpret_cast<const vec8 *>(qg + ks * 16 + g * 8);
+      if (qrow[qb] < p.sq && (!Sink || ks * 16 + g * 8 < p.d)) qf[qb][ks] = *reinterpret_cast<const vec8 *>(qg + ks * 16 + g * 8);
       else qf[qb][ks] = vec8{0};
     }
   }
@@ -131,7 +133,8 @@ __global__ void __launch_bounds__(NW * 64, NW * QB >= 16 ? 2 : (QB == 2 ? 1 : 2)
   // the descriptor's size); launch_fwd keeps head slices below 2 GiB so the sum cannot wrap.
   typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
   constexpr unsigned kRsrcFlags = 0x00020000;  // raw buffer, 32-bit data format
-  const unsigned k_bytes = idx::rsrc_bytes(sk, p.k_rs, D), v_bytes = idx::rsrc_bytes(sk, p.v_rs, D);
+  const int width = Sink ? p.d : D;
+  const unsigned k_bytes = idx::rsrc_bytes(sk, p.k_rs, width), v_bytes = idx::rsrc_bytes(sk, p.v_rs, width);
   const __amdgpu_buffer_rsrc_t k_rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(kg), 0, k_bytes, kRsrcFlags);
   const __amdgpu_buffer_rsrc_t v_rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(vg), 0, v_bytes, kRsrcFlags);
   unsigned k_vo[NP], v_vo[NP];
@@ -149,7 +152,7 @@ __global__ void __launch_bounds__(NW * 64, NW * QB >= 16 ? 2 : (QB == 2 ? 1 : 2)
 #pragma unroll
       for (int s = 0; s < NP; ++s) {
         const int row = kv0 + ld_r + s * RPP;
-        const bool seen = ld_on && row < st.hi && (row >= st.lo || row < st.sink);
+        const bool seen = ld_on && ld_c * 8 < p.d && row < st.hi && (row >= st.lo || row < st.sink);
         const u32x4 a = __builtin_amdgcn_raw_buffer_load_b128(k_rsrc, seen ? idx::chunk_offset(row, ld_c, p.k_rs) : 0xffffffffu, 0, 0);
         const u32x4 b = __builtin_amdgcn_raw_buffer_load_b128(v_rsrc, seen ? idx::chunk_offset(row, ld_c, p.v_rs) : 0xffffffffu, 0, 0);
         kreg[s] = uint4{a.x, a.y, a.z, a.w};
@@ -404,7 +407,7 @@ __global__ void __launch_bounds__(NW * 64, NW * QB >= 16 ? 2 : (QB == 2 ? 1 : 2)
         const int r = it * RPI + orow, q = wq0 + qb * 32 + r;
         uint4 v = *reinterpret_cast<const uint4 *>(&Ot[idx::ostage_read_offset(r, oc)]);
         if (r & 1) v = uint4{v.z, v.w, v.x, v.y};
-        if (q < p.sq)
+        if (q < p.sq && (!Sink || oc * 8 < p.d))
           *reinterpret_cast<uint4 *>(static_cast<T *>(p.o_w) + bi * p.o_bs + (int64_t)q * p.o_rs + hi * p.o_hs + oc * 8) = v;
       }
     } else if (qrow[qb] < p.sq) {
@@ -417,7 +420,7 @@ __global__ void __launch_bounds__(NW * 64, NW * QB >= 16 ? 2 : (QB == 2 ? 1 : 2)
           vec4 v;
 #pragma unroll
           for (int j = 0; j < 4; ++j) v[j] = (T)(o_acc[qb][db][i4 * 4 + j] * inv);
-          *reinterpret_cast<vec4 *>(og + db * 32 + i4 * 8 + g * 4) = v;
+          if (!Sink || db * 32 + i4 * 8 < p.d) *reinterpret_cast<vec4 *>(og + db * 32 + i4 * 8 + g * 4) = v;
         }
     }
     if (qrow[qb] < p.sq) {
@@ -428,37 +431,19 @@ __global__ void __launch_bounds__(NW * 64, NW * QB >= 16 ? 2 : (QB == 2 ? 1 : 2)
   }
 }
 
-// Number of key-axis splits for `n_wg` workgroups over `n_tiles` key tiles on 256 CUs: as the
-// reference's num_splits_heuristic (flash_api.cu:118-160) -- one split when the chip is already
-// 80 % full; otherwise the smallest count whose last round of workgroups is at least 85 % as
-// full as the best count's -- with at most 32 splits of at least eight tiles.
-inline int pick_splits(int n_wg, int n_tiles) {
-  constexpr int kCUs = 256;
-  if (n_wg >= 0.8f * kCUs) return 1;
-  const int max_splits = std::min(32, n_tiles / 8);
-  auto tiles_per = [&](int s) { return (n_tiles + s - 1) / s; };
-  auto eligible = [&](int s) { return s == 1 || tiles_per(s) != tiles_per(s - 1); };
-  auto eff = [&](int s) {
-    const float waves = float(n_wg * s) / kCUs;
-    return waves / std::ceil(waves);
-  };
-  float best = 0.f;
-  for (int s = 1; s <= max_splits; ++s)
-    if (eligible(s)) best = std::max(best, eff(s));
-  for (int s = 1; s <= max_splits; ++s)
-    if (eligible(s) && eff(s) >= 0.85f * best) return s;
-  return 1;
-}
-
 // Geometry: 8 waves of 32 rows, two waves per SIMD.  The kernel is written for 32*QB rows per
 // wave; QB = 2 halves the LDS traffic per MFMA, but either needs a whole SIMD per wave
 // (head_dim 128: slower, the compiler's schedule leaves the single wave stalled) or brought no
 // gain when it fits (head_dim 64), so QB = 1 is what is instantiated.
 template <int D> struct FwdGeom { static constexpr int QB = 1, NW = 8; };
 
-template <typename T, int D>
+// With sinks, NW = 4 (128 query rows) up to head_dim 64 when the grid of 256-row blocks would not fill
+// the chip: a block's list of tiles is shorter by what its window spans, and twice as many run (16
+// heads x 2 x 777 rows, window 256, D = 64: 23.0 -> 17.5 us).  At D = 128 a CU holds one workgroup, and
+// four waves alone take 3.0 us a tile against 2.1 of eight.
+template <typename T, int D, int NW>
 hipError_t launch_fwd_d(Params &p, hipStream_t stream) {
-  constexpr int QB = FwdGeom<D>::QB, NW = FwdGeom<D>::NW;
+  constexpr int QB = FwdGeom<D>::QB;
   constexpr int BM = 32 * QB * NW;
   p.n_mblocks = (p.sq + BM - 1) / BM;
   if (p.n_mblocks == 0) return hipSuccess;
@@ -468,11 +453,8 @@ hipError_t launch_fwd_d(Params &p, hipStream_t stream) {
   // enable it).  The partials live in the caller's workspace or, without one, in a
   // stream-ordered allocation; with neither: one split.
   const int n_wg = p.n_mblocks * p.b * p.h;
-  int n_tiles = (p.sk + kBN - 1) / kBN;
-  if (p.sink && p.wl >= 0 && p.wr >= 0) {  // with sinks the splits share out the list of tiles, which a window keeps short
-    const int64_t most = (int64_t)(std::min(p.n_sink, p.sk) + kBN - 1) / kBN + ((int64_t)p.wl + p.wr + BM) / kBN + 2;
-    n_tiles = (int)std::min<int64_t>(n_tiles, most);
-  }
+  // with sinks the splits share out the list of tiles, which a window keeps short
+  const int n_tiles = p.sink ? sink_tiles_bound(p, BM, kBN) : (p.sk + kBN - 1) / kBN;
   const int n_splits = pick_splits(n_wg, n_tiles);
   void *ws = nullptr;
   bool owned = false;
@@ -492,12 +474,16 @@ hipError_t launch_fwd_d(Params &p, hipStream_t stream) {
     p.ml_part = p.o_part + (size_t)n_splits * rows * D;
   }
   const dim3 grid((unsigned)n_wg, (unsigned)p.n_splits), block(NW * 64);
-  if (p.sink) FA_LAUNCH((flash_fwd_kernel<T, D, QB, NW, false, true>), grid, block, stream, p);
-  else if (p.seqlens_k) FA_LAUNCH((flash_fwd_kernel<T, D, QB, NW, true>), grid, block, stream, p);
-  else FA_LAUNCH((flash_fwd_kernel<T, D, QB, NW, false>), grid, block, stream, p);
+  if (p.sink) {
+    FA_LAUNCH((flash_fwd_kernel<T, D, QB, NW, false, true>), grid, block, stream, p);
+  } else if constexpr (NW == FwdGeom<D>::NW) {
+    if (p.seqlens_k) FA_LAUNCH((flash_fwd_kernel<T, D, QB, NW, true>), grid, block, stream, p);
+    else FA_LAUNCH((flash_fwd_kernel<T, D, QB, NW, false>), grid, block, stream, p);
+  }
   hipError_t e = hipGetLastError();
   if (ws) {
-    if (e == hipSuccess) e = launch_split_merge(p, std::is_same<T, _Float16>::value ? 1 : 2, stream);
+    constexpr int dtype = std::is_same<T, _Float16>::value ? 1 : 2;
+    if (e == hipSuccess) e = p.sink ? launch_sink_join(p, D, dtype, stream) : launch_split_merge(p, dtype, stream);
     if (owned) {
       const hipError_t fr = hipFreeAsync(ws, stream);
       if (e == hipSuccess) e = fr;
@@ -506,12 +492,19 @@ hipError_t launch_fwd_d(Params &p, hipStream_t stream) {
   return e;
 }
 
+template <typename T, int D>
+hipError_t launch_fwd_td(Params &p, hipStream_t stream) {
+  constexpr int NW = FwdGeom<D>::NW;
+  if (D <= 64 && p.sink && (int64_t)((p.sq + 32 * NW - 1) / (32 * NW)) * p.b * p.h < 256) return launch_fwd_d<T, D, D <= 64 ? NW / 2 : NW>(p, stream);
+  return launch_fwd_d<T, D, NW>(p, stream);
+}
+
 template <typename T>
 hipError_t launch_fwd_t(Params &p, hipStream_t stream) {
-  switch (p.d) {
-  case 32: return launch_fwd_d<T, 32>(p, stream);
-  case 64: return launch_fwd_d<T, 64>(p, stream);
-  case 128: return launch_fwd_d<T, 128>(p, stream);
+  switch (p.sink ? (p.d <= 32 ? 32 : p.d <= 64 ? 64 : 128) : p.d) {
+  case 32: return launch_fwd_td<T, 32>(p, stream);
+  case 64: return launch_fwd_td<T, 64>(p, stream);
+  case 128: return launch_fwd_td<T, 128>(p, stream);
   default: return hipErrorInvalidValue;
   }
 }
@@ -552,12 +545,13 @@ hipError_t launch_append_kv(const Params &p, int dtype, hipStream_t stream) {
 hipError_t launch_fwd(Params &p, int dtype, hipStream_t stream) {
   p.xcd_remap = idx::block_order_mode(p.b * p.h, p.wr);
   if (p.b * p.h == 0 || p.sq == 0) return hipSuccess;
-  if (!p.sink && decode_eligible(p)) return launch_decode(p, dtype, stream);
+  if (p.sink ? sink_few_rows(p) : decode_eligible(p)) return p.sink ? launch_sink_few_rows(p, dtype, stream) : launch_decode(p, dtype, stream);
   // the tuned kernel addresses a head's K and V rows through 32-bit buffer offsets
   // (the padded rows of the last tile and the tiles of look-ahead that the prologue always
   // requests are part of the span: their offsets must not wrap either)
   const int64_t kv_span = idx::fwd_stream_span_bytes(p.sk, std::max(p.k_rs, p.v_rs));
-  if (p.drop || (p.d != 32 && p.d != 64 && p.d != 128) || kv_span >= (int64_t(1) << 31)) return launch_fwd_anyd(p, dtype, stream);
+  const bool tuned = p.sink ? p.d <= 128 : p.d == 32 || p.d == 64 || p.d == 128;
+  if (p.drop || !tuned || kv_span >= (int64_t(1) << 31)) return launch_fwd_anyd(p, dtype, stream);
   return dtype == 1 ? launch_fwd_t<_Float16>(p, stream) : launch_fwd_t<__bf16>(p, stream);
 }
 

@@ -43,7 +43,7 @@ struct PagedParams {
   const void *q, *k, *v, *k_new, *v_new;  // the caches are written when k_new is given
   void *o;
   float *lse;                // [b, h, sq]
-  const int *seqlens;        // [b] keys in the cache before the call; < 0: the sequence is idle
+  const int *seqlens;        // [b] keys in the cache before the call; < 0: the sequence is idle; null: the capacity
   const float *w_in;         // [b, h_k, capacity]; null: from zero
   float *w_out;              // null: no weights
   Pages pages;
@@ -63,6 +63,7 @@ struct PagedParams {
 
   // keys of sequence bi after the call
   __device__ __forceinline__ int keys_of(int bi) const {
+    if (!seqlens) return pages.capacity();
     const int n = seqlens[bi];
     return n < 0 ? 0 : (int)min((int64_t)n + n_new, (int64_t)pages.capacity());
   }

@@ -90,7 +90,7 @@ __global__ void __launch_bounds__(kWaves * 64, D <= 128 ? 2 : 1) paged_kernel(co
   // (some entry of the table, or any word when there is none) and its result is not looked at
   // here: a test, or a choice between it and something else, would wait for it and with it for
   // every load in flight.
-  const int *table = p.pages.max_pages ? p.pages.table + (int64_t)bi * p.pages.max_pages : p.seqlens;
+  const int *table = p.pages.max_pages ? p.pages.table + (int64_t)bi * p.pages.max_pages : static_cast<const int *>(p.q);
   int number_next = 0, row_next = -1;
   auto locate = [&](int j) {
     const int key = idx::sink_tile(st, j) * kUnit + r32;
@@ -104,10 +104,11 @@ __global__ void __launch_bounds__(kWaves * 64, D <= 128 ? 2 : 1) paged_kernel(co
     const int lo = __builtin_amdgcn_ds_bpermute(src * 4, (int)v), hi = __builtin_amdgcn_ds_bpermute(src * 4, (int)(v >> 32));
     return (int64_t)(((uint64_t)(uint32_t)hi << 32) | (uint32_t)lo);
   };
-  // The rows of one pass lie on one page when the page size is a multiple of their number: their
+  // The rows of one pass lie on one page when the page size is a multiple of their number (or the
+  // cache is dense): their
   // address is then a scalar plus an offset that every pass shares, which costs the vector ALU
   // and the registers nothing.
-  const bool scalar_rows = p.pages.page % RPP == 0 && (uint64_t)p.pages.k_rs < (1 << 26) && (uint64_t)p.pages.v_rs < (1 << 26);
+  const bool scalar_rows = (p.pages.max_pages == 0 || p.pages.page % RPP == 0) && (uint64_t)p.pages.k_rs < (1 << 26) && (uint64_t)p.pages.v_rs < (1 << 26);
   const bool col_in = v_c * 8 < p.d;            // columns from head_dim up to D are zeros in the tiles
   const int v_col = col_in ? v_c * 8 : 0;       // their lanes load a column that exists and store nothing
   const uint32_t k_in = (uint32_t)(v_r * (uint32_t)p.pages.k_rs + v_col), v_in = (uint32_t)(v_r * (uint32_t)p.pages.v_rs + v_col);
@@ -333,37 +334,71 @@ __global__ void __launch_bounds__(kWaves * 64, D <= 128 ? 2 : 1) paged_kernel(co
   }
 }
 
-// joins the splits' partials of one (sequence, head, query row) per workgroup, one thread per output
-// element; n_splits <= 64, so lane s of every wave takes split s for the statistics
+// Joins the splits' partials: D / 4 threads take a row's columns, four each, and `groups` such sets of
+// threads share out the row's splits when rows are few and splits many (their sums meet in LDS);
+// else every set has a row of its own.  live: the number of splits that have written partials, or 0
+// for a paged call, where it follows from the row's sequence.
 template <typename T, int D>
-__global__ void __launch_bounds__(D < 64 ? 64 : D) paged_join_kernel(const PagedParams p) {
-  __shared__ float wgt[64];
-  const int64_t row = blockIdx.x, rows = (int64_t)p.b * p.h * p.sq;  // (sequence * h + head) * sq + query row
-  const int qi = (int)(row % p.sq), hq = (int)(row / p.sq % p.h), bi = (int)(row / p.sq / p.h);
-  const int n_units = min(p.units(p.keys_of(bi), (hq % (p.h / p.h_k) * p.sq + qi) / 32).n, p.max_units);
-  const int per = p.per_split(n_units), n_live = max(1, (n_units + per - 1) / per);
-  const int dcol = threadIdx.x < D ? threadIdx.x : D - 1, lane = threadIdx.x & 63;  // whole waves only
-  const bool has = lane < n_live;
-  const float m_s = has ? p.ml_part[(lane * rows + row) * 2] : -INFINITY;
-  const float l_s = has ? p.ml_part[(lane * rows + row) * 2 + 1] : 0.f;
-  float m_all = m_s;
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) m_all = fmaxf(m_all, __shfl_xor(m_all, off, 64));
-  const float m_ref = m_all == -INFINITY ? 0.f : m_all;
-  const float w_s = exp2_fast((m_s - m_ref) * p.scale_log2);  // 0 for a split that saw no key
-  float l_all = w_s * l_s;
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) l_all += __shfl_xor(l_all, off, 64);
-  if (threadIdx.x < 64) wgt[threadIdx.x] = w_s;
-  __syncthreads();
-  float acc = 0.f;
-  const float *op = p.o_part + row * D + dcol;
+__global__ void __launch_bounds__(256) join_kernel(const PagedParams p, int groups, int live) {
+  constexpr int TPR = D / 4, SETS = 256 / TPR;
+  __shared__ float4 acc_s[256];
+  __shared__ float l_s[SETS];
+  const int tid = threadIdx.x, set = tid / TPR, col = tid % TPR * 4;
+  const int64_t rows = (int64_t)p.b * p.h * p.sq;
+  const int64_t row = (int64_t)blockIdx.x * (SETS / groups) + set / groups, r = row < rows ? row : rows - 1;  // (sequence * h + head) * sq + query row
+  const int share = set % groups;
+  const int qi = (int)(r % p.sq), hq = (int)(r / p.sq % p.h), bi = (int)(r / p.sq / p.h);
+  int n_live = live;
+  if (live == 0) {
+    const int n_units = min(p.units(p.keys_of(bi), (hq % (p.h / p.h_k) * p.sq + qi) / 32).n, p.max_units), per = p.per_split(n_units);
+    n_live = max(1, (n_units + per - 1) / per);
+  }
+  const float2 *ml = reinterpret_cast<const float2 *>(p.ml_part) + r;
+  const float *op = p.o_part + r * D + col;
+  float m_all = -INFINITY;
 #pragma unroll 8
-  for (int s = 0; s < n_live; ++s) acc += wgt[s] * op[s * rows * D];
-  const bool empty = l_all == 0.f;
-  T *og = static_cast<T *>(p.o) + bi * p.o_bs + (int64_t)qi * p.o_rs + hq * p.o_hs;
-  if (threadIdx.x < p.d) og[dcol] = (T)(empty ? 0.f : acc / l_all);
-  if (threadIdx.x == 0) p.lse[row] = empty ? INFINITY : m_all * p.scale + log2_fast(l_all) * kLn2;
+  for (int s = 0; s < n_live; ++s) m_all = fmaxf(m_all, ml[s * rows].x);
+  const float m_ref = m_all == -INFINITY ? 0.f : m_all;
+  float l = 0.f;
+  float4 t = float4{0, 0, 0, 0};
+#pragma unroll 4
+  for (int s = share; s < n_live; s += groups) {
+    const float2 x = ml[s * rows];
+    const float w = exp2_fast((x.x - m_ref) * p.scale_log2);  // 0 for a split that saw no key
+    const float4 o = *reinterpret_cast<const float4 *>(op + s * rows * D);
+    l += w * x.y;
+    t.x += w * o.x; t.y += w * o.y; t.z += w * o.z; t.w += w * o.w;
+  }
+  if (groups > 1) {
+    acc_s[tid] = t;
+    if (tid % TPR == 0) l_s[set] = l;
+    __syncthreads();
+    if (share > 0) return;
+    for (int x = 1; x < groups; ++x) {
+      const float4 o = acc_s[tid + x * TPR];
+      l += l_s[set + x];
+      t.x += o.x; t.y += o.y; t.z += o.z; t.w += o.w;
+    }
+  }
+  if (row >= rows) return;
+  const bool empty = l == 0.f;
+  const float inv = empty ? 0.f : 1.f / l;
+  typedef T vec4 __attribute__((ext_vector_type(4)));
+  if (col < p.d)
+    *reinterpret_cast<vec4 *>(static_cast<T *>(p.o) + bi * p.o_bs + (int64_t)qi * p.o_rs + hq * p.o_hs + col) =
+        vec4{(T)(t.x * inv), (T)(t.y * inv), (T)(t.z * inv), (T)(t.w * inv)};
+  if (col == 0) p.lse[row] = empty ? INFINITY : m_all * p.scale + log2_fast(l) * kLn2;
+}
+
+template <typename T, int D>
+hipError_t join_td(const PagedParams &p, int live, hipStream_t stream) {
+  constexpr int SETS = 256 / (D / 4);
+  const int64_t rows = (int64_t)p.b * p.h * p.sq;
+  int groups = 1;  // more as long as every CU has a workgroup's rows less than once
+  while (groups < SETS && groups < p.n_splits && rows * groups < 256 * SETS) groups *= 2;
+  const int per = SETS / groups;
+  FA_LAUNCH((join_kernel<T, D>), dim3((unsigned)((rows + per - 1) / per)), dim3(256), stream, p, groups, live);
+  return hipGetLastError();
 }
 
 // weights_out[key] = weights_in[key] (0 for a row appended by this call) + sum of P over the columns of
@@ -448,8 +483,7 @@ hipError_t paged_td(PagedParams &p, hipStream_t stream) {
     e = hipGetLastError();
   }
   if (e == hipSuccess && p.o_part) {
-    FA_LAUNCH((paged_join_kernel<T, D>), dim3((unsigned)rows), dim3(D < 64 ? 64 : D), stream, p);
-    e = hipGetLastError();
+    e = join_td<T, D>(p, 0, stream);
   }
   if (e == hipSuccess && p.w_out) {
     FA_LAUNCH((paged_weights_kernel), dim3((unsigned)((int64_t)((p.pages.capacity() + 255) / 256) * p.b * p.h_k)), dim3(256), stream, p);
@@ -486,10 +520,47 @@ hipError_t launch_paged(PagedParams &p, int dtype, hipStream_t stream) {
   // per split 16 / 32 / 64 / 128, kernel time: 64 x 8192 keys, 8 heads, D = 128: 368 / 351 / 346 /
   // 340 us, 1000..8191 keys: 231 / 212 / 211 / 238 with the join; 8 x 8192: 55 / 52 / 56 / 87.
   p.min_units = (int)std::min<int64_t>(64, std::max<int64_t>(kWaves, (p.max_units * base + 511) / 512));
-  p.n_splits = p.max_units <= 2 * kWaves ? 1 : (int)std::min<int64_t>(64, (p.max_units + p.min_units - 1) / p.min_units);
+  // up to three units a wave are read before a second launch would have joined two workgroups
+  p.n_splits = p.max_units <= 3 * kWaves ? 1 : (int)std::min<int64_t>(64, (p.max_units + p.min_units - 1) / p.min_units);
   // the attention kernel appends when one workgroup's tile covers all columns and its window reaches the first new row
   p.fuse_append = p.n_new > 0 && p.n_ct == 1 && (p.wl < 0 || p.n_new <= (int64_t)p.sq + p.wl);
   return dtype == 1 ? paged_t<_Float16>(p, stream) : paged_t<__bf16>(p, stream);
+}
+
+// A few rows per key/value head (two column tiles) against the dense keys of a flash_attn_sink_fwd
+// call: streaming the keys beats a block of 128 or 256 rows that is mostly empty.
+bool sink_few_rows(const Params &p) { return (int64_t)(p.h / p.h_k) * p.sq <= 64 && p.sk >= 1; }
+
+hipError_t launch_sink_join(const Params &p, int width, int dtype, hipStream_t stream) {
+  PagedParams a{};
+  a.o = p.o_w; a.lse = p.lse;
+  a.o_bs = p.o_bs; a.o_rs = p.o_rs; a.o_hs = p.o_hs;
+  a.b = p.b; a.h = p.h; a.h_k = p.h_k; a.d = p.d; a.sq = p.sq;
+  a.scale = p.scale; a.scale_log2 = p.scale_log2;
+  a.n_splits = p.n_splits;
+  a.o_part = p.o_part; a.ml_part = p.ml_part;
+  auto go = [&](auto t) {
+    using T = decltype(t);
+    return width == 32 ? join_td<T, 32>(a, p.n_splits, stream) : width == 64 ? join_td<T, 64>(a, p.n_splits, stream)
+         : width == 128 ? join_td<T, 128>(a, p.n_splits, stream) : join_td<T, 256>(a, p.n_splits, stream);
+  };
+  return dtype == 1 ? go((_Float16)0) : go((__bf16)0);
+}
+
+hipError_t launch_sink_few_rows(const Params &p, int dtype, hipStream_t stream) {
+  PagedParams a{};
+  a.q = p.q; a.k = p.k; a.v = p.v; a.o = p.o_w; a.lse = p.lse;
+  set_page(a.pages, p.sk);
+  a.pages.num_pages = p.b;
+  a.pages.k_ps = p.k_bs; a.pages.k_rs = p.k_rs; a.pages.k_hs = p.k_hs;
+  a.pages.v_ps = p.v_bs; a.pages.v_rs = p.v_rs; a.pages.v_hs = p.v_hs;
+  a.q_bs = p.q_bs; a.q_rs = p.q_rs; a.q_hs = p.q_hs;
+  a.o_bs = p.o_bs; a.o_rs = p.o_rs; a.o_hs = p.o_hs;
+  a.b = p.b; a.h = p.h; a.h_k = p.h_k; a.d = p.d; a.sq = p.sq;
+  a.scale = p.scale; a.scale_log2 = p.scale_log2;
+  a.wl = p.wl; a.wr = p.wr; a.n_sink = p.n_sink;
+  a.ws = p.ws; a.ws_bytes = p.ws_bytes; a.ws_query = p.ws_query;
+  return launch_paged(a, dtype, stream);
 }
 
 }  // namespace fa

@@ -237,11 +237,11 @@ hipError_t sink_dkdv_t(const Params &p, const SinkArgs &a, hipStream_t stream) {
   return sink_dkdv_td<T, 256>(p, a, stream);
 }
 
-// two workgroups for every CU, at least four items a wave, at most 64 shares
+// two workgroups for every CU, at least two items a wave, at most 64 shares
 int sink_shares(const Params &p) {
   const int64_t base = (int64_t)p.b * p.h_k * ((p.n_sink + kSinkKeys - 1) / kSinkKeys);
   const int64_t items = (int64_t)(p.h / p.h_k) * ((p.sq + kSinkRows - 1) / kSinkRows);
-  return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>((512 + base - 1) / base, items / (4 * kSinkWaves)), 64));
+  return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>((512 + base - 1) / base, items / (2 * kSinkWaves)), 64));
 }
 
 }  // namespace
