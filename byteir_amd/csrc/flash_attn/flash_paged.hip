@@ -77,7 +77,6 @@ __global__ void __launch_bounds__(kWaves * 64, D <= 128 ? 2 : 1) paged_kernel(co
   const T *kg = static_cast<const T *>(p.k) + hk * p.pages.k_hs;
   const T *vg = static_cast<const T *>(p.v) + hk * p.pages.v_hs;
   T *Kt = reinterpret_cast<T *>(lds[wave]), *Vt = Kt + kUnit * KS;
-  uint4 kn[NPV], vn[NPV];
   const int v_c = lane % CPR, v_r = lane / CPR;
   typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
   // rows from new0 on come from k_new / v_new instead of the cache and are written to it
@@ -91,14 +90,13 @@ __global__ void __launch_bounds__(kWaves * 64, D <= 128 ? 2 : 1) paged_kernel(co
   // here: a test, or a choice between it and something else, would wait for it and with it for
   // every load in flight.
   const int *table = p.pages.max_pages ? p.pages.table + (int64_t)bi * p.pages.max_pages : static_cast<const int *>(p.q);
-  int number_next = 0, row_next = -1;
+  struct Place { int number, row; };
   auto locate = [&](int j) {
     const int key = idx::sink_tile(st, j) * kUnit + r32;
     const bool seen = key < st.hi && (key >= st.lo || key < st.sink);
     int at = 0, row = key;
     if (p.pages.max_pages) at = p.pages.index(seen ? key : 0, row);
-    number_next = table[at];
-    row_next = seen ? row : -1;
+    return Place{table[at], seen ? row : -1};
   };
   auto from_lane = [&](int64_t v, int src) {  // lane src's value
     const int lo = __builtin_amdgcn_ds_bpermute(src * 4, (int)v), hi = __builtin_amdgcn_ds_bpermute(src * 4, (int)(v >> 32));
@@ -113,57 +111,60 @@ __global__ void __launch_bounds__(kWaves * 64, D <= 128 ? 2 : 1) paged_kernel(co
   const int v_col = col_in ? v_c * 8 : 0;       // their lanes load a column that exists and store nothing
   const uint32_t k_in = (uint32_t)(v_r * (uint32_t)p.pages.k_rs + v_col), v_in = (uint32_t)(v_r * (uint32_t)p.pages.v_rs + v_col);
   // Unit j, located, into the staging registers, when all its 32 rows are to be read from the
-  // cache; -> which of its rows exist.  A unit with rows that are not (the ends of a sequence or
+  // cache.  A unit with rows that are not (the ends of a sequence or
   // window, absent pages, new rows) is read by store_unit instead: keeping it in flight as well would
   // cost the registers that the LDS reads of the loop need to run ahead of the MFMAs.
-  int pg_cur = 0, row_cur = -1;
-  bool staged = false;
-  auto load_unit = [&](int j) -> uint32_t {
-    const int pg_next = p.pages.max_pages ? number_next : bi;
-    const uint32_t there = (uint32_t)__builtin_amdgcn_ballot_w64(row_next >= 0 && p.pages.present(pg_next));
-    pg_cur = pg_next;
-    row_cur = row_next;
+  struct Stage {
+    uint4 k[NPV], v[NPV];
+    int pg = 0, row = -1;
+    uint32_t there = 0;   // which of the unit's rows exist
+    bool staged = false;
+  };
+  auto load_unit = [&](int j, const Place &at, Stage &u) {
+    const int pg_next = p.pages.max_pages ? at.number : bi, row_next = at.row;
+    u.there = (uint32_t)__builtin_amdgcn_ballot_w64(row_next >= 0 && p.pages.present(pg_next));
+    u.pg = pg_next;
+    u.row = row_next;
     int vr = v_r;
     FA_PIN(vr);  // what the uncommon paths derive from it is computed there, not kept in registers over the loop
-    staged = there == 0xffffffffu && idx::sink_tile(st, j) * kUnit + kUnit <= new0;
-    if (staged && scalar_rows) {
+    u.staged = u.there == 0xffffffffu && idx::sink_tile(st, j) * kUnit + kUnit <= new0;
+    if (u.staged && scalar_rows) {
 #pragma unroll
       for (int s = 0; s < NPV; ++s) {
         const int64_t pg = __builtin_amdgcn_readlane(pg_next, s * RPP), row = __builtin_amdgcn_readlane(row_next, s * RPP);
         const u32x4 a = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(kg + pg * p.pages.k_ps + row * p.pages.k_rs + k_in));
         const u32x4 b = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(vg + pg * p.pages.v_ps + row * p.pages.v_rs + v_in));
-        kn[s] = uint4{a.x, a.y, a.z, a.w};
-        vn[s] = uint4{b.x, b.y, b.z, b.w};
+        u.k[s] = uint4{a.x, a.y, a.z, a.w};
+        u.v[s] = uint4{b.x, b.y, b.z, b.w};
       }
-    } else if (staged) {
+    } else if (u.staged) {
       const int64_t k_lane = pg_next * p.pages.k_ps + row_next * p.pages.k_rs, v_lane = pg_next * p.pages.v_ps + row_next * p.pages.v_rs;
 #pragma unroll
       for (int s = 0; s < NPV; ++s) {
         const int64_t ko = from_lane(k_lane, s * RPP + vr), vo = from_lane(v_lane, s * RPP + vr);
         const u32x4 a = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(kg + ko + v_col));
         const u32x4 b = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(vg + vo + v_col));
-        kn[s] = uint4{a.x, a.y, a.z, a.w};
-        vn[s] = uint4{b.x, b.y, b.z, b.w};
+        u.k[s] = uint4{a.x, a.y, a.z, a.w};
+        u.v[s] = uint4{b.x, b.y, b.z, b.w};
       }
     }
-    return there;
   };
-  auto store_unit = [&](int j, uint32_t there) {  // unit j into the wave's tiles
-    if (!staged) {
+  auto store_unit = [&](int j, Stage &u) {  // unit j into the wave's tiles
+    if (!u.staged) {
       const int kv0 = idx::sink_tile(st, j) * kUnit;
       int vr = v_r;
       FA_PIN(vr);
-      const int64_t k_lane = pg_cur * p.pages.k_ps + row_cur * p.pages.k_rs, v_lane = pg_cur * p.pages.v_ps + row_cur * p.pages.v_rs;
+      const int64_t k_lane = u.pg * p.pages.k_ps + u.row * p.pages.k_rs, v_lane = u.pg * p.pages.v_ps + u.row * p.pages.v_rs;
 #pragma unroll
       for (int s = 0; s < NPV; ++s) {
         const int r = s * RPP + vr, key = kv0 + r;
         const int64_t ko = from_lane(k_lane, r), vo = from_lane(v_lane, r);
         const bool fresh = key >= new0;
-        kn[s] = uint4{0, 0, 0, 0};  // a row that nobody sees: 0 * finite stays finite in P V
-        vn[s] = uint4{0, 0, 0, 0};
-        if (((there >> r) & 1u) & col_in) {
-          kn[s] = *reinterpret_cast<const uint4 *>((fresh ? kng + (int64_t)(key - new0) * p.kn_rs : kg + ko) + v_col);
-          vn[s] = *reinterpret_cast<const uint4 *>((fresh ? vng + (int64_t)(key - new0) * p.vn_rs : vg + vo) + v_col);
+        u.k[s] = uint4{0, 0, 0, 0};  // a row that nobody sees: 0 * finite stays finite in P V
+        u.v[s] = uint4{0, 0, 0, 0};
+        if (((u.there >> r) & 1u) & col_in) {
+          u.k[s] = *reinterpret_cast<const uint4 *>((fresh ? kng + (int64_t)(key - new0) * p.kn_rs : kg + ko) + v_col);
+          u.v[s] = *reinterpret_cast<const uint4 *>((fresh ? vng + (int64_t)(key - new0) * p.vn_rs : vg + vo) + v_col);
         }
       }
       if (kv0 + kUnit > new0) {
@@ -171,9 +172,9 @@ __global__ void __launch_bounds__(kWaves * 64, D <= 128 ? 2 : 1) paged_kernel(co
         for (int s = 0; s < NPV; ++s) {
           const int r = s * RPP + vr;
           const int64_t ko = from_lane(k_lane, r), vo = from_lane(v_lane, r);
-          if (((there >> r) & 1u) && col_in && kv0 + r >= new0) {
-            *reinterpret_cast<uint4 *>(const_cast<T *>(kg) + ko + v_col) = kn[s];
-            *reinterpret_cast<uint4 *>(const_cast<T *>(vg) + vo + v_col) = vn[s];
+          if (((u.there >> r) & 1u) && col_in && kv0 + r >= new0) {
+            *reinterpret_cast<uint4 *>(const_cast<T *>(kg) + ko + v_col) = u.k[s];
+            *reinterpret_cast<uint4 *>(const_cast<T *>(vg) + vo + v_col) = u.v[s];
           }
         }
       }
@@ -181,8 +182,8 @@ __global__ void __launch_bounds__(kWaves * 64, D <= 128 ? 2 : 1) paged_kernel(co
     if (col_in) {
 #pragma unroll
       for (int s = 0; s < NPV; ++s) {
-        *reinterpret_cast<uint4 *>(&Kt[(s * RPP + v_r) * KS + v_c * 8]) = kn[s];
-        *reinterpret_cast<uint4 *>(&Vt[(s * RPP + v_r) * VS + v_c * 8]) = vn[s];
+        *reinterpret_cast<uint4 *>(&Kt[(s * RPP + v_r) * KS + v_c * 8]) = u.k[s];
+        *reinterpret_cast<uint4 *>(&Vt[(s * RPP + v_r) * VS + v_c * 8]) = u.v[s];
       }
     }
     FA_WAVE_SYNC();  // the wave's own tile: written by all its lanes, read across lanes, no workgroup barrier
@@ -204,24 +205,29 @@ __global__ void __launch_bounds__(kWaves * 64, D <= 128 ? 2 : 1) paged_kernel(co
   float m_run = -INFINITY, m_scaled = 0.f, l_run = 0.f;
   const float c = p.scale_log2;
 
+  // One unit in flight beside the one in LDS.  (Two, where the registers allow it: no faster; 16 heads,
+  // D = 64, 64 x 8192 keys 376 against 380 us.)
+  Stage stage;
+  Place next{0, -1};
+  const int first = u0 + wave;
   uint32_t there = 0;
-  if (u0 + wave < u1) {
-    locate(u0 + wave);
-    there = load_unit(u0 + wave);
-    locate(min(u0 + wave + kWaves, u1 - 1));
-    store_unit(u0 + wave, there);
+  if (first < u1) {
+    const Place p0 = locate(first);
+    next = locate(min(first + kWaves, u1 - 1));
+    load_unit(first, p0, stage);
+    store_unit(first, stage);
+    there = stage.there;
   }
   // The Q fragments are consumed here: the wait for their loads would otherwise stand before the first
   // MFMA of every unit and drain the loads of the next one too.
 #pragma unroll
   for (int ks = 0; ks < D / 16; ++ks) FA_PIN(qf[ks]);
-  for (int j = u0 + wave; j < u1; j += kWaves) {
-    const bool has_next = j + kWaves < u1;
-    uint32_t there_next = 0;
-    if (has_next) {
-      there_next = load_unit(j + kWaves);
-      locate(min(j + 2 * kWaves, u1 - 1));
-    }
+  for (int j = first; j < u1; j += kWaves) {
+    // the table before the rows: loads return in order, and waiting for the number must not mean
+    // waiting for the rows requested after it
+    const Place after = locate(min(j + 2 * kWaves, u1 - 1));
+    if (j + kWaves < u1) load_unit(j + kWaves, next, stage);
+    next = after;
     float16v s = float16v{0};
 #pragma unroll
     for (int ks = 0; ks < D / 16; ++ks)
@@ -278,8 +284,10 @@ __global__ void __launch_bounds__(kWaves * 64, D <= 128 ? 2 : 1) paged_kernel(co
       for (int db = 0; db < D / 32; ++db)
         o_acc[db] = Traits<T>::mfma(lds_read_operand_tr<T>(Vt, VS, w * 16, db * 32), pb, o_acc[db]);
     }
-    if (has_next) store_unit(j + kWaves, there_next);  // after every read of unit j in program order
-    there = there_next;
+    if (j + kWaves < u1) {
+      store_unit(j + kWaves, stage);  // after every read of unit j in program order
+      there = stage.there;
+    }
   }
 
   // ---- the four waves' partials joined through LDS (each wave writes into its own region) ----
@@ -402,28 +410,40 @@ hipError_t join_td(const PagedParams &p, int live, hipStream_t stream) {
 }
 
 // weights_out[key] = weights_in[key] (0 for a row appended by this call) + sum of P over the columns of
-// the key/value head, in column order; a thread per key, keys behind the last one are left alone
+// the key/value head, in column order; a thread per 4 keys (of one unit), keys behind the last one
+// are left alone
 __global__ void __launch_bounds__(256) paged_weights_kernel(const PagedParams p) {
-  const int blocks = (p.pages.capacity() + 255) / 256;
+  const int cap = p.pages.capacity(), blocks = (cap + 1023) / 1024;
   const int bhk = blockIdx.x / blocks, bi = bhk / p.h_k, hk = bhk % p.h_k;
-  const int key = blockIdx.x % blocks * 256 + threadIdx.x, sk = p.keys_of(bi);
+  const int key = (blockIdx.x % blocks * 256 + threadIdx.x) * 4, sk = p.keys_of(bi);
   if (key >= sk) return;
-  const int group = p.h / p.h_k, n_cols = group * p.sq;
-  const int64_t at = (int64_t)bhk * p.pages.capacity() + key;
-  float w = p.w_in && key < p.seqlens[bi] ? p.w_in[at] : 0.f;
-  const int tile = key / kUnit;
+  const int group = p.h / p.h_k, n_cols = group * p.sq, tile = key / kUnit, old = p.seqlens[bi];
+  const int64_t at = (int64_t)bhk * cap + key;
+  const int n = min(4, sk - key);
+  float w[4];
+#pragma unroll
+  for (int y = 0; y < 4; ++y) w[y] = p.w_in && y < n && key + y < old ? p.w_in[at + y] : 0.f;
+  const float *lse = p.lse + ((int64_t)bi * p.h + hk * group) * p.sq;  // column n's at n
   for (int ct = 0; ct < p.n_ct; ++ct) {
     const idx::SinkTiles st = p.units(sk, ct);
-    const int j = tile < st.ns ? tile : tile - st.n0 + st.ns;  // the unit that holds the key
+    const int j = tile < st.ns ? tile : tile - st.n0 + st.ns;  // the unit that holds the keys
     if ((tile >= st.ns && tile < st.n0) || j >= min(st.n, p.max_units)) continue;
     const int c1 = min(n_cols, (ct + 1) * 32);
-    for (int n = ct * 32; n < c1; ++n) {
-      const float s = p.s_part[(((int64_t)bhk * n_cols + n) * p.max_units + j) * kUnit + key % kUnit];
-      const float lse = p.lse[((int64_t)bi * p.h + hk * group + n / p.sq) * p.sq + n % p.sq];
-      w += s == -INFINITY ? 0.f : exp2_fast(fmaf(s, p.scale_log2, -lse * kLog2e));
+    const float *sp = p.s_part + ((int64_t)bhk * n_cols * p.max_units + j) * kUnit + key % kUnit;
+#pragma unroll 4
+    for (int c = ct * 32; c < c1; ++c) {
+      const float4 s = *reinterpret_cast<const float4 *>(sp + (int64_t)c * p.max_units * kUnit);
+      const float l = -lse[c] * kLog2e;
+      // -inf: a key that the column does not see, also where the column sees none (lse = +inf)
+      w[0] += s.x == -INFINITY ? 0.f : exp2_fast(fmaf(s.x, p.scale_log2, l));
+      w[1] += s.y == -INFINITY ? 0.f : exp2_fast(fmaf(s.y, p.scale_log2, l));
+      w[2] += s.z == -INFINITY ? 0.f : exp2_fast(fmaf(s.z, p.scale_log2, l));
+      w[3] += s.w == -INFINITY ? 0.f : exp2_fast(fmaf(s.w, p.scale_log2, l));
     }
   }
-  p.w_out[at] = w;
+#pragma unroll
+  for (int y = 0; y < 4; ++y)
+    if (y < n) p.w_out[at + y] = w[y];
 }
 
 // the new rows into the cache, 16 bytes a thread; rows behind the capacity or on an absent page are dropped
@@ -486,7 +506,7 @@ hipError_t paged_td(PagedParams &p, hipStream_t stream) {
     e = join_td<T, D>(p, 0, stream);
   }
   if (e == hipSuccess && p.w_out) {
-    FA_LAUNCH((paged_weights_kernel), dim3((unsigned)((int64_t)((p.pages.capacity() + 255) / 256) * p.b * p.h_k)), dim3(256), stream, p);
+    FA_LAUNCH((paged_weights_kernel), dim3((unsigned)((int64_t)((p.pages.capacity() + 1023) / 1024) * p.b * p.h_k)), dim3(256), stream, p);
     e = hipGetLastError();
   }
   if (owned) {
