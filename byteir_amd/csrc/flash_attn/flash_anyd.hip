@@ -563,8 +563,12 @@ __global__ void __launch_bounds__(256, DR <= 64 ? 2 : 1) dkdv_anyd_kernel(const 
 }
 
 // ---- backward 3: dQ ---------------------------------------------------------------------------------
-template <typename T, int DR, bool Drop, bool Sink = false>
-__global__ void __launch_bounds__(256, (DR <= 96 || (DR == 128 && !Drop)) ? 2 : 1) dq_anyd_kernel(const Params p) {
+// Exact: D = dO . O, which the kernel takes from the stored O itself, carries the roundings of that O (its
+// own and those of P in P V).  With e = sum_j P (dP - D), which would be zero for the D of these P
+// and dP, D + e has none of them; dQ is corrected by -e scale sum_j P K (one more product that shares
+// the K fragments of dS K), and D + e is written for the dK / dV kernel.
+template <typename T, int DR, bool Drop, bool Sink = false, bool Exact = false>
+__global__ void __launch_bounds__(256, (Exact ? DR <= 64 : DR <= 96 || (DR == 128 && !Drop)) ? 2 : 1) dq_anyd_kernel(const Params p) {
   using vec8 = typename Traits<T>::vec8;
   constexpr int KS = Pad<DR>::kPlain;  // K tile: plain and transposed reads
   constexpr int VS = Pad<DR>::kPlain;  // V tile: plain reads only
@@ -606,11 +610,25 @@ __global__ void __launch_bounds__(256, (DR <= 96 || (DR == 128 && !Drop)) ? 2 : 
   float lse_l = INFINITY, dsm_l = 0.f;
   if (qrow < p.sq) {
     lse_l = p.lse[((int64_t)bi * p.h + hi) * p.sq + qrow] * kLog2e;
-    dsm_l = p.dsoftmax[((int64_t)bi * p.h + hi) * p.sq_rounded + qrow];
+    if (!Exact) dsm_l = p.dsoftmax[((int64_t)bi * p.h + hi) * p.sq_rounded + qrow];
   }
-  float16v dq_acc[DR / 32];
+  if constexpr (Exact) {
+    const T *og = static_cast<const T *>(p.o) + bi * p.o_bs + (int64_t)qrow * p.o_rs + hi * p.o_hs;
 #pragma unroll
-  for (int i = 0; i < DR / 32; ++i) dq_acc[i] = float16v{0};
+    for (int ks = 0; ks < DR / 16; ++ks) {
+      const vec8 of = load_frag<T>(og, qrow < p.sq, ks * 16 + g * 8, p.d);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) dsm_l += (float)of[j] * (float)dof[ks][j];
+    }
+    dsm_l += partner32(dsm_l);  // the other half of the columns
+  }
+  float err = 0.f;                             // Exact: this lane's part of e
+  float16v dq_acc[DR / 32], pk_acc[Exact ? DR / 32 : 1];
+#pragma unroll
+  for (int i = 0; i < DR / 32; ++i) {
+    dq_acc[i] = float16v{0};
+    if constexpr (Exact) pk_acc[i] = float16v{0};
+  }
   const float c = p.scale_log2;
   DropCtx drop;
   if constexpr (Drop) drop.init(p, bh);
@@ -644,7 +662,7 @@ __global__ void __launch_bounds__(256, (DR <= 96 || (DR == 128 && !Drop)) ? 2 : 
     const bool skip = kv0 >= w_hi_last || (kv0 + kTile <= w_lo_first && !(Sink && kv0 < p.n_sink));
     if (!skip) {
       const bool need_mask = kv0 + kTile > w_hi_first || (kv0 < w_lo_last && !(Sink && kv0 + kTile <= p.n_sink));
-      float16v s[2], dp[2];
+      float16v s[2], dp[2];  // Exact: dp becomes P
 #pragma unroll
       for (int kvb = 0; kvb < 2; ++kvb) {
         s[kvb] = float16v{0};
@@ -670,6 +688,10 @@ __global__ void __launch_bounds__(256, (DR <= 96 || (DR == 128 && !Drop)) ? 2 : 
           }
           const bool kept = !Drop || ((keep >> i) & 1u);
           s[kvb][i] = pe * ((kept ? dp[kvb][i] : 0.f) - dsm_l);  // dS^T
+          if constexpr (Exact) {
+            err += s[kvb][i];
+            dp[kvb][i] = pe;
+          }
         }
       }
 #pragma unroll
@@ -678,10 +700,17 @@ __global__ void __launch_bounds__(256, (DR <= 96 || (DR == 128 && !Drop)) ? 2 : 
 #pragma unroll
         for (int j = 0; j < 8; ++j) f[j] = s[w >> 1][(w & 1) * 8 + j];
         const vec8 dsb = pack8<T>(f);
+        vec8 pb;
+        if constexpr (Exact) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) f[j] = dp[w >> 1][(w & 1) * 8 + j];
+          pb = pack8<T>(f);
+        }
 #pragma unroll
         for (int db = 0; db < DR / 32; ++db) {
           const vec8 a = lds_read_operand_tr<T>(Ks, KS, w * 16, db * 32);
           dq_acc[db] = Traits<T>::mfma(a, dsb, dq_acc[db]);
+          if constexpr (Exact) pk_acc[db] = Traits<T>::mfma(a, pb, pk_acc[db]);
         }
       }
     }
@@ -692,6 +721,14 @@ __global__ void __launch_bounds__(256, (DR <= 96 || (DR == 128 && !Drop)) ? 2 : 
     }
   }
 
+  if constexpr (Exact) {
+    err += partner32(err);  // the other half of the keys
+    if (qrow < p.sq && g == 0) p.dsoftmax[((int64_t)bi * p.h + hi) * p.sq_rounded + qrow] = dsm_l + err;
+#pragma unroll
+    for (int db = 0; db < DR / 32; ++db)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) dq_acc[db][i] -= err * pk_acc[db][i];
+  }
   if (qrow < p.sq) {
     T *dqg = static_cast<T *>(p.dq) + bi * p.q_bs + (int64_t)qrow * p.q_rs + hi * p.q_hs;
 #pragma unroll
@@ -763,7 +800,7 @@ hipError_t bwd_anyd_d(const Params &p, hipStream_t stream) {
       if (e != hipSuccess) return e;
     }
   }
-  if (p.n_mblocks > 0 && !p.ws_query) {
+  if (p.n_mblocks > 0 && !p.ws_query && !p.have_dq) {
     if (p.sink) FA_LAUNCH((dq_anyd_kernel<T, DR, false, true>), gq, block, stream, p);
     else if (p.drop) FA_LAUNCH((dq_anyd_kernel<T, DR, true>), gq, block, stream, p);
     else FA_LAUNCH((dq_anyd_kernel<T, DR, false>), gq, block, stream, p);
@@ -784,7 +821,7 @@ hipError_t fwd_anyd_t(Params &p, hipStream_t stream) {
 template <typename T>
 hipError_t bwd_anyd_t(const Params &p, hipStream_t stream) {
   const int64_t rows = (int64_t)p.b * p.h * p.sq;
-  if (rows > 0 && !p.ws_query) FA_LAUNCH((dot_do_o_anyd_kernel<T>), dim3((unsigned)((rows + 7) / 8)), dim3(256), stream, p);
+  if (rows > 0 && !p.ws_query && !p.have_dq) FA_LAUNCH((dot_do_o_anyd_kernel<T>), dim3((unsigned)((rows + 7) / 8)), dim3(256), stream, p);
   if (p.d <= 32) return bwd_anyd_d<T, 32>(p, stream);
   if (p.d <= 64) return bwd_anyd_d<T, 64>(p, stream);
   if (p.d <= 96) return bwd_anyd_d<T, 96>(p, stream);
@@ -817,6 +854,29 @@ hipError_t launch_dq_anyd128(const Params &p, int dtype, hipStream_t stream) {
   } else if (dtype == 1) FA_LAUNCH((dq_anyd_kernel<_Float16, 128, false>), grid, block, stream, pq);
   else FA_LAUNCH((dq_anyd_kernel<__bf16, 128, false>), grid, block, stream, pq);
   return hipGetLastError();
+}
+
+template <typename T, int DR>
+hipError_t dq_exact_d(const Params &p, hipStream_t stream) {
+  FA_LAUNCH((dq_anyd_kernel<T, DR, false, true, true>), dim3((unsigned)(p.n_mblocks * p.b * p.h)), dim3(256), stream, p);
+  return hipGetLastError();
+}
+template <typename T>
+hipError_t dq_exact_t(const Params &p, hipStream_t stream) {
+  if (p.d <= 32) return dq_exact_d<T, 32>(p, stream);
+  if (p.d <= 64) return dq_exact_d<T, 64>(p, stream);
+  if (p.d <= 96) return dq_exact_d<T, 96>(p, stream);
+  if (p.d <= 128) return dq_exact_d<T, 128>(p, stream);
+  if (p.d <= 192) return dq_exact_d<T, 192>(p, stream);
+  return dq_exact_d<T, 256>(p, stream);
+}
+
+// dQ and D of a flash_attn_sink_bwd call without the roundings that D takes from the stored O
+hipError_t launch_dq_exact(const Params &p, int dtype, hipStream_t stream) {
+  Params pq = p;
+  pq.n_mblocks = (p.sq + kRows - 1) / kRows;
+  if (pq.n_mblocks == 0) return hipSuccess;
+  return dtype == 1 ? dq_exact_t<_Float16>(pq, stream) : dq_exact_t<__bf16>(pq, stream);
 }
 
 hipError_t launch_bwd_anyd(Params &p, int dtype, hipStream_t stream) {

@@ -777,7 +777,7 @@ __global__ void __launch_bounds__(256) group_sum_kernel(const Params p, const vo
 template <typename T, int D>
 hipError_t launch_bwd_td(const Params &p, hipStream_t stream) {
   const int64_t rows = (int64_t)p.b * p.h * p.sq;
-  if (rows > 0 && !p.ws_query) {
+  if (rows > 0 && !p.ws_query && !p.have_dq) {
     constexpr int RPB = 256 / (D / 8);
     FA_LAUNCH((dot_do_o_kernel<T, D>), dim3((unsigned)((rows + RPB - 1) / RPB)), dim3(256), stream, p);
   }
@@ -802,6 +802,7 @@ hipError_t launch_bwd_td(const Params &p, hipStream_t stream) {
     const hipError_t e = launch_group_sum(p, split, D, std::is_same<T, _Float16>::value ? 1 : 2, stream);
     if (e != hipSuccess) return e;
   }
+  if (p.have_dq) return hipGetLastError();
   Params pq = p;
   pq.n_mblocks = (p.sq + kQBlock - 1) / kQBlock;
   if constexpr (D == 128) {
@@ -875,6 +876,15 @@ hipError_t launch_bwd(Params &p, int dtype, hipStream_t stream) {
   if (hipError_t e = launch_bwd_all(plan, dtype, nullptr)) return e;
   base = (base + 15) & ~(size_t)15;
   if (p.ws_query) { *p.ws_query = base + sink_dkdv_bytes(p); return hipSuccess; }
+  // The roundings that D = dO . O takes from the stored O are divided among the keys a row sees; where
+  // those are few (512: a window, or all the keys there are) dQ comes first, from the kernel that
+  // takes them out, and leaves D for the others (16 heads, 777 rows, window 256, D = 64: dQ off by
+  // 1.50 roundings rms against 64 bits with D as it is, 1.42 so).
+  const int64_t seen = p.wl < 0 || p.wr < 0 ? p.sk : std::min<int64_t>(p.sk, (int64_t)p.wl + p.wr + 1 + p.n_sink);
+  if (seen <= 512) {
+    if (hipError_t e = launch_dq_exact(p, dtype, stream)) return e;
+    p.have_dq = 1;
+  }
   if (hipError_t e = launch_bwd_all(p, dtype, stream)) return e;
   const bool rest = p.ws && p.ws_bytes > base;
   return launch_sink_dkdv(p, dtype, rest ? static_cast<char *>(p.ws) + base : nullptr, rest ? p.ws_bytes - base : 0, stream);
