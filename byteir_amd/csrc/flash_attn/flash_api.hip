@@ -144,9 +144,10 @@ int sink_args(const void *extra_args, const Blob &a, fa::Params &p) {
   if (a.b * a.h_k * ((n_sink < a.seqlen_k ? n_sink : a.seqlen_k) / 32 + 1) > (1 << 22)) return fail("problem too large for 32-bit tile indices");
   p.sink = 1;
   p.n_sink = (int)(n_sink < a.seqlen_k ? n_sink : a.seqlen_k);
-  // a window wider than the keys is no window; this also keeps row + window inside 32 bits
-  if (a.window_size_left >= a.seqlen_k + a.seqlen_q) p.wl = -1;
-  if (a.window_size_right >= a.seqlen_k + a.seqlen_q) p.wr = -1;
+  // rows, keys and windows are added in 32 bits; a side that reaches past every key is no bound
+  if (a.seqlen_q + a.seqlen_k > (1 << 29)) return fail("problem too large for 32-bit tile indices");
+  if (a.window_size_left >= a.seqlen_k) p.wl = -1;
+  if (a.window_size_right >= a.seqlen_q) p.wr = -1;
   return 0;
 }
 
@@ -332,9 +333,10 @@ int paged_impl(void **tensors, const void *extra_args, int dtype, const Scratch 
   p.b = (int)b; p.h = (int)h; p.h_k = (int)h_k; p.d = (int)d; p.sq = (int)sq; p.n_new = (int)n_new;
   p.scale = scale;
   p.scale_log2 = (float)(scale * M_LOG2E);
-  // a window wider than everything is no window
-  p.wl = wl < 0 || wl >= cap + sq ? -1 : (int)wl;
-  p.wr = wr < 0 || wr >= cap + sq ? -1 : (int)wr;
+  // rows, keys and windows are added in 32 bits; a side that reaches past every key is no bound
+  if (cap + sq + n_new > (1 << 30)) return fail("problem too large for 32-bit tile indices");
+  p.wl = wl < 0 || wl >= cap ? -1 : (int)wl;
+  p.wr = wr < 0 || wr >= sq ? -1 : (int)wr;
   p.n_sink = (int)(n_sink < cap ? n_sink : cap);
   p.ws = sc.ws; p.ws_bytes = sc.ws_bytes; p.ws_query = sc.query;
   // the threads of a launch are counted in 32 bits

@@ -542,6 +542,8 @@ hipError_t launch_paged(PagedParams &p, int dtype, hipStream_t stream) {
   p.min_units = (int)std::min<int64_t>(64, std::max<int64_t>(kWaves, (p.max_units * base + 511) / 512));
   // up to three units a wave are read before a second launch would have joined two workgroups
   p.n_splits = p.max_units <= 3 * kWaves ? 1 : (int)std::min<int64_t>(64, (p.max_units + p.min_units - 1) / p.min_units);
+  // the threads of a launch are counted in 32 bits
+  if (base * p.n_splits > (1 << 23) || (int64_t)p.b * p.h * p.sq > (1 << 24)) p.n_splits = 1;
   // the attention kernel appends when one workgroup's tile covers all columns and its window reaches the first new row
   p.fuse_append = p.n_new > 0 && p.n_ct == 1 && (p.wl < 0 || p.n_new <= (int64_t)p.sq + p.wl);
   return dtype == 1 ? paged_t<_Float16>(p, stream) : paged_t<__bf16>(p, stream);

@@ -618,6 +618,8 @@ def _plan_evict(k, v, weights, seqlens_k, block_table, k_out, v_out, out_table, 
         k, v, weights, seqlens_k, block_table, k_out, v_out, out_table, weights_out, seqlens_out, kept)
     if (k_out is None) != (v_out is None):
         raise ValueError("k_out and v_out must be given together")
+    if budget < 1:
+        raise ValueError(f"budget {budget} is not positive")
     _half(k, v, k_out, v_out)
     if k.shape != v.shape:
         raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} do not fit together")

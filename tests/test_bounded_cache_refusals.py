@@ -39,6 +39,25 @@ def test_sink_refusals(change, why):
         E.sink_bwd(do, q, k, v, torch.zeros_like(q), lse, args["scale"], (4, 0), args["n_sink"])
 
 
+def test_sink_refuses_lengths_that_32_bits_do_not_add():
+    q, k, v, _ = sink_tensors()
+    blob = ops.pack_flash_sink_args(q, k, v, q, 0.5, (4, 0), 4)
+    at = 17 * 8 + 4  # seqlen_q, seqlen_k
+    for sq, sk in ((1 << 29, 8), (8, 1 << 29), (1 << 28, (1 << 28) + 1)):
+        with pytest.raises(E.EmuFault, match="too large"):
+            E._call("sink_fwd", [None] * 7, blob[:at] + struct.pack("<2q", sq, sk) + blob[at + 16:], H)
+
+
+def test_windows_wider_than_everything_are_none():
+    """Window sides at the limits of their field."""
+    gen = torch.Generator().manual_seed(1)
+    q, k, v = (torch.randn(1, n, 2, 32, generator=gen).half() for n in (40, 70, 70))
+    want = E.sink_fwd(q, k, v, 0.2, (-1, -1), 3)
+    for window in ((70, 40), ((1 << 31) - 1, (1 << 31) - 1), (69, 39)):
+        got = E.sink_fwd(q, k, v, 0.2, window, 3)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
 def test_sink_refuses_dropout_bad_types_and_null_tensors():
     q, k, v, _ = sink_tensors()
     o, lse = torch.zeros_like(q), torch.zeros(1, 2, 8)
@@ -65,7 +84,8 @@ def paged_blob(**change):
     (dict(max_pages=1 << 28), r"more than 2\^30 rows"), (dict(max_pages=0, pages=1), "2 sequences in a cache of 1"), (dict(sq=-1), "bad seqlen_q"),
     (dict(new=-1), "seqlen_knew"), (dict(sink=-1), "n_sink"), (dict(mode=3), "weights mode"), (dict(scale=0.0), "not positive"),
     (dict(scale=float("inf")), "not positive"), (dict(sq=0), "new rows without query rows"), (dict(sq=1 << 29), "too large"),
-    (dict(b=1 << 22, h=1024, hk=1024), "too large"), (dict(pages=(1 << 31)), "bad page counts"),
+    (dict(b=1 << 22, h=1024, hk=1024), "too large"), (dict(pages=(1 << 31)), "bad page counts"), (dict(page=1 << 28), "too large"),
+    (dict(new=1 << 30), "too large"),
 ])
 def test_paged_refusals(change, why):
     # the reason comes before any tensor is looked at
@@ -150,6 +170,8 @@ def test_python_calls_check_their_tensors():
     raises(p, q, kp, kp, table, n, 0.5, weights_out=torch.zeros(1, 2, 63), match="weights_out must be")
     w, e = torch.zeros(1, 2, 64), ops.flash_attn_evict
     raises(e, kp, kp, w, n, 10, block_table=table, match="device tensor required")
+    raises(e, kp, kp, w, n, 0, block_table=table, match="budget 0 is not positive")
+    raises(e, kp, kp, w, n, -3, block_table=table, match="budget -3 is not positive")
     raises(e, kp, kp, w, n, 10, match="1 sequences, but a dense cache of 8")
     raises(e, kp, kp, w, n, 10, block_table=table, k_out=kp, match="given together")
     raises(e, kp, kp, w, n, 10, block_table=table, out_table=table, match="out_table without k_out")
