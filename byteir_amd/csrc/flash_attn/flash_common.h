@@ -192,6 +192,7 @@ struct Params {
   float scale, scale_log2;
   int wl, wr;                         // window sizes after normalisation; < 0 = unbounded
   int sink;                           // 1: a flash_attn_sink_* call (the Sink kernels, also when n_sink is 0)
+  int pack;                           // forward with sinks: log2 of the query heads that share a workgroup
   int n_sink;                         // the first n_sink keys stay visible outside the window
   int have_dq;                        // backward: 1: dq and dsoftmax have been written (launch_dq_exact)
   int kv_lo, kv_hi;                   // backward: the keys that some query row can see (dK/dV kernels load no others)

@@ -40,7 +40,11 @@ constexpr float kRescaleSlack = 8.0f;
 // first, then the window's, as one list of tiles walked by the same loop; a tile row that none
 // of the workgroup's query rows can see is read as zeros, whatever it holds.  Here D may exceed
 // head_dim: the columns behind it are zeros on the way in and not written (a head_dim of 80 at
-// D = 128 takes two thirds of the time of the generic kernel at 96 columns).
+// D = 128 takes two thirds of the time of the generic kernel at 96 columns).  And here 2^p.pack
+// query heads of one key/value head share a workgroup: its waves take their heads in turn and
+// the block has that many times fewer rows, so that its tiles span the window and little more
+// (32 heads on 8, window 1024: 18 tiles and the sinks' for 64 rows of four heads against 21 for 256
+// of one; D = 128, 8192 rows: 231 against 205 us).
 template <typename T, int D, int QB, int NW, bool VarK, bool Sink = false>
 __global__ void __launch_bounds__(NW * 64, NW * QB >= 16 ? 2 : (QB == 2 ? 1 : 2)) flash_fwd_kernel(const Params p) {
   constexpr int kThreads = NW * 64;
@@ -63,13 +67,15 @@ __global__ void __launch_bounds__(NW * 64, NW * QB >= 16 ? 2 : (QB == 2 ? 1 : 2)
   // first within an XCD, then the second longest of every one, ...: longest-first list
   // scheduling, which fills the CUs evenly over the causal triangle (measured 216 -> 178 us on
   // fp16 causal b4 h32 s2048 d128) at the price of more (batch, head) pairs in flight per L2.
-  const idx::BlockId blk = idx::decode_block((int)blockIdx.x, p.xcd_remap, p.b * p.h, p.n_mblocks);
+  const int pack = Sink ? p.pack : 0, n_heads = p.h >> pack;  // heads, or sets of them
+  const idx::BlockId blk = idx::decode_block((int)blockIdx.x, p.xcd_remap, p.b * n_heads, p.n_mblocks);
   const int bh = blk.bh, m_block = p.n_mblocks - 1 - blk.blk;  // longest (causal) blocks first
-  const int bi = bh / p.h, hi = bh % p.h, hk = hi / (p.h / p.h_k);
+  const int bi = bh / n_heads, hi0 = (bh % n_heads) << pack, hi = hi0 + (wave & ((1 << pack) - 1)), hk = hi0 / (p.h / p.h_k);
   int sk = p.sk;
   if constexpr (VarK) sk = min(p.sk, p.seqlens_k[bi] + p.seqlen_knew);
-  const int m0 = m_block * kBM;
-  const int wq0 = m0 + wave * 32 * QB;
+  const int bm = kBM >> pack;  // rows of the block
+  const int m0 = m_block * bm;
+  const int wq0 = m0 + (wave >> pack) * 32 * QB;
 
   int qrow[QB], lo_lim[QB], hi_lim[QB];
   // limits of each half's first and last row bound what the half can see
@@ -86,7 +92,7 @@ __global__ void __launch_bounds__(NW * 64, NW * QB >= 16 ? 2 : (QB == 2 ? 1 : 2)
   int n_min, n_max;  // Sink: positions in the list of tiles
   idx::SinkTiles st{};
   if constexpr (Sink) {
-    st = idx::sink_tile_range(p.sq, sk, p.wl, p.wr, p.n_sink, m0, kBM, kBN);
+    st = idx::sink_tile_range(p.sq, sk, p.wl, p.wr, p.n_sink, m0, bm, kBN);
     n_min = 0;
     n_max = st.n;
   } else {
@@ -445,16 +451,21 @@ template <typename T, int D, int NW>
 hipError_t launch_fwd_d(Params &p, hipStream_t stream) {
   constexpr int QB = FwdGeom<D>::QB;
   constexpr int BM = 32 * QB * NW;
-  p.n_mblocks = (p.sq + BM - 1) / BM;
+  p.pack = 0;
+  if (p.sink)
+    while ((2 << p.pack) <= NW && p.h / p.h_k % (2 << p.pack) == 0) ++p.pack;
+  const int bm = BM >> p.pack, n_heads = p.h >> p.pack;
+  p.n_mblocks = (p.sq + bm - 1) / bm;
   if (p.n_mblocks == 0) return hipSuccess;
+  if (p.sink) p.xcd_remap = idx::block_order_mode(p.b * n_heads, p.wr);
   // Few query blocks and many keys (a long prompt chunk of one sequence): split the key axis over
   // workgroups until the chip is full, at least eight tiles per split (the reference's
   // num_splits_heuristic has the same aim, flash_api.cu:118-160, but its entry points never
   // enable it).  The partials live in the caller's workspace or, without one, in a
   // stream-ordered allocation; with neither: one split.
-  const int n_wg = p.n_mblocks * p.b * p.h;
+  const int n_wg = p.n_mblocks * p.b * n_heads;
   // with sinks the splits share out the list of tiles, which a window keeps short
-  const int n_tiles = p.sink ? sink_tiles_bound(p, BM, kBN) : (p.sk + kBN - 1) / kBN;
+  const int n_tiles = p.sink ? sink_tiles_bound(p, bm, kBN) : (p.sk + kBN - 1) / kBN;
   const int n_splits = pick_splits(n_wg, n_tiles);
   void *ws = nullptr;
   bool owned = false;
