@@ -579,9 +579,10 @@ __global__ void __launch_bounds__(256, (Exact ? DR <= 64 : DR <= 96 || (DR == 12
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int r32 = lane & 31, g = lane >> 5;
   int m_block, bh;
-  block_of(p, p.n_mblocks, true, m_block, bh);
-  const int bi = bh / p.h, hi = bh % p.h;
-  const int m0 = m_block * kRows, wq0 = m0 + wave * 32, qrow = wq0 + r32;
+  const int pack = Sink ? p.pack : 0, n_heads = p.h >> pack, n_rows = kRows >> pack;  // as in flash_fwd.hip
+  block_of(p, p.n_mblocks, true, m_block, bh, p.b * n_heads);
+  const int bi = bh / n_heads, hi = ((bh % n_heads) << pack) + (wave & ((1 << pack) - 1));
+  const int m0 = m_block * n_rows, wq0 = m0 + (wave >> pack) * 32, qrow = wq0 + r32;
 
   int lo_lim, hi_lim, w_lo_first, w_hi_first, w_lo_last, w_hi_last, b_lo, b_hi, t0, t1;
   row_limits(p, qrow, lo_lim, hi_lim);
@@ -590,7 +591,7 @@ __global__ void __launch_bounds__(256, (Exact ? DR <= 64 : DR <= 96 || (DR == 12
   row_limits(p, m0, b_lo, t0);
   row_limits(p, m0 + kRows - 1, t1, b_hi);
   idx::SinkTiles st{};
-  if constexpr (Sink) st = idx::sink_tile_range(p.sq, p.sk, p.wl, p.wr, p.n_sink, m0, kRows, kTile);
+  if constexpr (Sink) st = idx::sink_tile_range(p.sq, p.sk, p.wl, p.wr, p.n_sink, m0, n_rows, kTile);
   const int n_min = Sink ? 0 : b_lo / kTile;
   const int n_max = Sink ? st.n : b_hi > 0 ? (b_hi + kTile - 1) / kTile : 0;
   auto tile_kv0 = [&](int t) { return (Sink ? idx::sink_tile(st, t) : t) * kTile; };  // first key of the t-th tile
@@ -780,6 +781,18 @@ hipError_t fwd_anyd_d(Params &p, hipStream_t stream) {
   return hipGetLastError();
 }
 
+template <typename T, int DR, bool Exact>
+hipError_t dq_sink_d(const Params &p, hipStream_t stream) {
+  Params pq = p;
+  pq.pack = head_pack(p, 4);
+  const int n_heads = p.h >> pq.pack, rows = kRows >> pq.pack;
+  pq.n_mblocks = (p.sq + rows - 1) / rows;
+  if (pq.n_mblocks == 0) return hipSuccess;
+  pq.xcd_remap = idx::block_order_mode(p.b * n_heads, p.wr);
+  FA_LAUNCH((dq_anyd_kernel<T, DR, false, true, Exact>), dim3((unsigned)(pq.n_mblocks * p.b * n_heads)), dim3(256), stream, pq);
+  return hipGetLastError();
+}
+
 template <typename T, int DR>
 hipError_t bwd_anyd_d(const Params &p, hipStream_t stream) {
   const dim3 gk((unsigned)(p.n_nblocks * p.b * p.h_k)), gq((unsigned)(p.n_mblocks * p.b * p.h)), block(256);
@@ -801,8 +814,8 @@ hipError_t bwd_anyd_d(const Params &p, hipStream_t stream) {
     }
   }
   if (p.n_mblocks > 0 && !p.ws_query && !p.have_dq) {
-    if (p.sink) FA_LAUNCH((dq_anyd_kernel<T, DR, false, true>), gq, block, stream, p);
-    else if (p.drop) FA_LAUNCH((dq_anyd_kernel<T, DR, true>), gq, block, stream, p);
+    if (p.sink) return dq_sink_d<T, DR, false>(p, stream);
+    if (p.drop) FA_LAUNCH((dq_anyd_kernel<T, DR, true>), gq, block, stream, p);
     else FA_LAUNCH((dq_anyd_kernel<T, DR, false>), gq, block, stream, p);
   }
   return hipGetLastError();
@@ -848,35 +861,25 @@ hipError_t launch_dq_anyd128(const Params &p, int dtype, hipStream_t stream) {
   pq.n_mblocks = (p.sq + kRows - 1) / kRows;
   if (pq.n_mblocks == 0) return hipSuccess;
   const dim3 grid((unsigned)(pq.n_mblocks * p.b * p.h)), block(256);
-  if (p.sink) {
-    if (dtype == 1) FA_LAUNCH((dq_anyd_kernel<_Float16, 128, false, true>), grid, block, stream, pq);
-    else FA_LAUNCH((dq_anyd_kernel<__bf16, 128, false, true>), grid, block, stream, pq);
-  } else if (dtype == 1) FA_LAUNCH((dq_anyd_kernel<_Float16, 128, false>), grid, block, stream, pq);
+  if (p.sink) return dtype == 1 ? dq_sink_d<_Float16, 128, false>(p, stream) : dq_sink_d<__bf16, 128, false>(p, stream);
+  if (dtype == 1) FA_LAUNCH((dq_anyd_kernel<_Float16, 128, false>), grid, block, stream, pq);
   else FA_LAUNCH((dq_anyd_kernel<__bf16, 128, false>), grid, block, stream, pq);
   return hipGetLastError();
 }
 
-template <typename T, int DR>
-hipError_t dq_exact_d(const Params &p, hipStream_t stream) {
-  FA_LAUNCH((dq_anyd_kernel<T, DR, false, true, true>), dim3((unsigned)(p.n_mblocks * p.b * p.h)), dim3(256), stream, p);
-  return hipGetLastError();
-}
 template <typename T>
 hipError_t dq_exact_t(const Params &p, hipStream_t stream) {
-  if (p.d <= 32) return dq_exact_d<T, 32>(p, stream);
-  if (p.d <= 64) return dq_exact_d<T, 64>(p, stream);
-  if (p.d <= 96) return dq_exact_d<T, 96>(p, stream);
-  if (p.d <= 128) return dq_exact_d<T, 128>(p, stream);
-  if (p.d <= 192) return dq_exact_d<T, 192>(p, stream);
-  return dq_exact_d<T, 256>(p, stream);
+  if (p.d <= 32) return dq_sink_d<T, 32, true>(p, stream);
+  if (p.d <= 64) return dq_sink_d<T, 64, true>(p, stream);
+  if (p.d <= 96) return dq_sink_d<T, 96, true>(p, stream);
+  if (p.d <= 128) return dq_sink_d<T, 128, true>(p, stream);
+  if (p.d <= 192) return dq_sink_d<T, 192, true>(p, stream);
+  return dq_sink_d<T, 256, true>(p, stream);
 }
 
 // dQ and D of a flash_attn_sink_bwd call without the roundings that D takes from the stored O
 hipError_t launch_dq_exact(const Params &p, int dtype, hipStream_t stream) {
-  Params pq = p;
-  pq.n_mblocks = (p.sq + kRows - 1) / kRows;
-  if (pq.n_mblocks == 0) return hipSuccess;
-  return dtype == 1 ? dq_exact_t<_Float16>(pq, stream) : dq_exact_t<__bf16>(pq, stream);
+  return dtype == 1 ? dq_exact_t<_Float16>(p, stream) : dq_exact_t<__bf16>(p, stream);
 }
 
 hipError_t launch_bwd_anyd(Params &p, int dtype, hipStream_t stream) {

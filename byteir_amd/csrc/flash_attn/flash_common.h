@@ -192,7 +192,7 @@ struct Params {
   float scale, scale_log2;
   int wl, wr;                         // window sizes after normalisation; < 0 = unbounded
   int sink;                           // 1: a flash_attn_sink_* call (the Sink kernels, also when n_sink is 0)
-  int pack;                           // forward with sinks: log2 of the query heads that share a workgroup
+  int pack;                           // with sinks: log2 of the query heads that share a workgroup
   int n_sink;                         // the first n_sink keys stay visible outside the window
   int have_dq;                        // backward: 1: dq and dsoftmax have been written (launch_dq_exact)
   int kv_lo, kv_hi;                   // backward: the keys that some query row can see (dK/dV kernels load no others)
@@ -310,6 +310,12 @@ bool sink_few_rows(const Params &p);
 hipError_t launch_sink_join(const Params &p, int width, int dtype, hipStream_t stream);
 hipError_t launch_sink_few_rows(const Params &p, int dtype, hipStream_t stream);
 // most key tiles of `bn` rows that a block of `bm` query rows of a flash_attn_sink_fwd call visits
+// log2 of the query heads of a key/value head that can share a workgroup of `waves` waves
+inline int head_pack(const Params &p, int waves) {
+  int n = 0;
+  while ((2 << n) <= waves && p.h / p.h_k % (2 << n) == 0) ++n;
+  return n;
+}
 inline int sink_tiles_bound(const Params &p, int bm, int bn) {
   const int all = (p.sk + bn - 1) / bn;
   if (p.wl < 0 || p.wr < 0) return all;

@@ -451,9 +451,7 @@ template <typename T, int D, int NW>
 hipError_t launch_fwd_d(Params &p, hipStream_t stream) {
   constexpr int QB = FwdGeom<D>::QB;
   constexpr int BM = 32 * QB * NW;
-  p.pack = 0;
-  if (p.sink)
-    while ((2 << p.pack) <= NW && p.h / p.h_k % (2 << p.pack) == 0) ++p.pack;
+  p.pack = p.sink ? head_pack(p, NW) : 0;
   const int bm = BM >> p.pack, n_heads = p.h >> p.pack;
   p.n_mblocks = (p.sq + bm - 1) / bm;
   if (p.n_mblocks == 0) return hipSuccess;
