@@ -867,19 +867,30 @@ hipError_t launch_dq_anyd128(const Params &p, int dtype, hipStream_t stream) {
   return hipGetLastError();
 }
 
-template <typename T>
-hipError_t dq_exact_t(const Params &p, hipStream_t stream) {
-  if (p.d <= 32) return dq_sink_d<T, 32, true>(p, stream);
-  if (p.d <= 64) return dq_sink_d<T, 64, true>(p, stream);
-  if (p.d <= 96) return dq_sink_d<T, 96, true>(p, stream);
-  if (p.d <= 128) return dq_sink_d<T, 128, true>(p, stream);
-  if (p.d <= 192) return dq_sink_d<T, 192, true>(p, stream);
-  return dq_sink_d<T, 256, true>(p, stream);
+template <typename T, bool Exact>
+hipError_t dq_sink_t(const Params &p, hipStream_t stream) {
+  if (p.d <= 32) return dq_sink_d<T, 32, Exact>(p, stream);
+  if (p.d <= 64) return dq_sink_d<T, 64, Exact>(p, stream);
+  if (p.d <= 96) return dq_sink_d<T, 96, Exact>(p, stream);
+  if (p.d <= 128) return dq_sink_d<T, 128, Exact>(p, stream);
+  if (p.d <= 192) return dq_sink_d<T, 192, Exact>(p, stream);
+  return dq_sink_d<T, 256, Exact>(p, stream);
+}
+
+// D and dQ of a flash_attn_sink_bwd call, every head_dim
+hipError_t launch_dq_any(const Params &p, int dtype, hipStream_t stream) {
+  const int64_t rows = (int64_t)p.b * p.h * p.sq;
+  if (rows == 0) return hipSuccess;
+  const dim3 grid((unsigned)((rows + 7) / 8));
+  if (dtype == 1) FA_LAUNCH((dot_do_o_anyd_kernel<_Float16>), grid, dim3(256), stream, p);
+  else FA_LAUNCH((dot_do_o_anyd_kernel<__bf16>), grid, dim3(256), stream, p);
+  if (hipError_t e = hipGetLastError()) return e;
+  return dtype == 1 ? dq_sink_t<_Float16, false>(p, stream) : dq_sink_t<__bf16, false>(p, stream);
 }
 
 // dQ and D of a flash_attn_sink_bwd call without the roundings that D takes from the stored O
 hipError_t launch_dq_exact(const Params &p, int dtype, hipStream_t stream) {
-  return dtype == 1 ? dq_exact_t<_Float16>(p, stream) : dq_exact_t<__bf16>(p, stream);
+  return dtype == 1 ? dq_sink_t<_Float16, true>(p, stream) : dq_sink_t<__bf16, true>(p, stream);
 }
 
 hipError_t launch_bwd_anyd(Params &p, int dtype, hipStream_t stream) {

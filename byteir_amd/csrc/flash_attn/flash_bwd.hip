@@ -71,11 +71,13 @@ struct TileLoader {
   // backward).  The running offsets travel in the vector offset, which is what the hardware
   // checks against the descriptor's size; the launcher keeps a (batch, head) slice below
   // 2 GiB so they cannot wrap.
-  __device__ __forceinline__ void start(const T *base, int64_t row_stride, int row0, int n_rows) {
+  // width < D: the columns from there on read as zeros (their offsets start, and stay, beyond every
+  // slice the launcher admits).
+  __device__ __forceinline__ void start(const T *base, int64_t row_stride, int row0, int n_rows, int width = D) {
     const int c = threadIdx.x % CPR, r = threadIdx.x / CPR;
-    rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(base), 0, idx::rsrc_bytes(n_rows, row_stride, D), 0x00020000);
+    rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(base), 0, idx::rsrc_bytes(n_rows, row_stride, width), 0x00020000);
 #pragma unroll
-    for (int s = 0; s < NP; ++s) vo[s] = idx::chunk_offset(row0 + r + s * RPP, c, row_stride);
+    for (int s = 0; s < NP; ++s) vo[s] = c * 8 < width ? idx::chunk_offset(row0 + r + s * RPP, c, row_stride) : 0x80000000u;
     tile_b = idx::tile_bytes(ROWS, row_stride);
   }
   // the next tile into a register set of the caller's (two tiles in flight at a workgroup's start)
@@ -137,7 +139,8 @@ struct TileLoader {
 // and the first step accumulates a zero P / dS.
 // KB: 32-key blocks per wave; the workgroup covers 128*KB keys and every Q / dO fragment read
 // from LDS feeds KB MFMAs.
-template <typename T, int D, int KB>
+// Any: head_dim may be smaller than D; the columns behind it are zeros on the way in and not written.
+template <typename T, int D, int KB, bool Any = false>
 __global__ void __launch_bounds__(256, (D <= 64 && KB == 1) ? 2 : 1) dkdv_kernel(const Params p) {
   using vec8 = typename Traits<T>::vec8;
   // Tiles are read both plainly and transposed.  A stride of 4*odd banks keeps the plain reads
@@ -181,7 +184,7 @@ __global__ void __launch_bounds__(256, (D <= 64 && KB == 1) ? 2 : 1) dkdv_kernel
     const T *vg = static_cast<const T *>(p.v) + bi * p.v_bs + (int64_t)kvcol[kb] * p.v_rs + hkv * p.v_hs;
 #pragma unroll
     for (int ks = 0; ks < D / 16; ++ks) {
-      if (kvcol[kb] < p.kv_hi && kvcol[kb] >= p.kv_lo) {
+      if (kvcol[kb] < p.kv_hi && kvcol[kb] >= p.kv_lo && (!Any || ks * 16 + g * 8 < p.d)) {
         kf[kb][ks] = *reinterpret_cast<const vec8 *>(kg + ks * 16 + g * 8);
         vf[kb][ks] = *reinterpret_cast<const vec8 *>(vg + ks * 16 + g * 8);
       } else {
@@ -357,8 +360,8 @@ __global__ void __launch_bounds__(256, (D <= 64 && KB == 1) ? 2 : 1) dkdv_kernel
   dog = static_cast<const T *>(p.dout) + bi * p.o_bs + hi * p.o_hs;
   lse_g = p.lse + ((int64_t)bi * p.h + hi) * p.sq;
   dsm_g = p.dsoftmax + ((int64_t)bi * p.h + hi) * p.sq_rounded;
-  lq.start(qg, p.q_rs, m_min * kQTile, p.sq);
-  ldo.start(dog, p.o_rs, m_min * kQTile, p.sq);
+  lq.start(qg, p.q_rs, m_min * kQTile, p.sq, Any ? p.d : D);
+  ldo.start(dog, p.o_rs, m_min * kQTile, p.sq, Any ? p.d : D);
   q_next = m_min * kQTile + tid;
   if (gq > 0) {
     __syncthreads();  // every wave has left the previous head's last tile
@@ -441,6 +444,7 @@ __global__ void __launch_bounds__(256, (D <= 64 && KB == 1) ? 2 : 1) dkdv_kernel
         for (int db = 0; db < D / 32; ++db)
 #pragma unroll
           for (int i4 = 0; i4 < 4; ++i4) {
+            if (Any && db * 32 + i4 * 8 >= p.d) continue;
             const float16v &a = dk_acc[kb][db], &b = dv_acc[kb][db];
             *reinterpret_cast<float4 *>(dkp + db * 32 + i4 * 8 + g * 4) =
                 float4{a[i4 * 4] * p.scale, a[i4 * 4 + 1] * p.scale, a[i4 * 4 + 2] * p.scale, a[i4 * 4 + 3] * p.scale};
@@ -483,7 +487,7 @@ __global__ void __launch_bounds__(256, (D <= 64 && KB == 1) ? 2 : 1) dkdv_kernel
       uint4 a = *reinterpret_cast<const uint4 *>(&Kt[idx::ostage_read_offset(r, oc)]);
       uint4 b = *reinterpret_cast<const uint4 *>(&Vt[idx::ostage_read_offset(r, oc)]);
       if (r & 1) { a = uint4{a.z, a.w, a.x, a.y}; b = uint4{b.z, b.w, b.x, b.y}; }
-      if (kv < p.sk) {
+      if (kv < p.sk && (!Any || oc * 8 < p.d)) {
         *reinterpret_cast<uint4 *>(static_cast<T *>(p.dk) + bi * p.dk_bs + (int64_t)kv * p.dk_rs + hk * p.dk_hs + oc * 8) = a;
         *reinterpret_cast<uint4 *>(static_cast<T *>(p.dv) + bi * p.dv_bs + (int64_t)kv * p.dv_rs + hk * p.dv_hs + oc * 8) = b;
       }
@@ -506,6 +510,7 @@ __global__ void __launch_bounds__(256, (D <= 64 && KB == 1) ? 2 : 1) dkdv_kernel
             a[j] = (T)(dk_acc[kb][db][i4 * 4 + j] * p.scale);
             b[j] = (T)(dv_acc[kb][db][i4 * 4 + j]);
           }
+          if (Any && db * 32 + i4 * 8 >= p.d) continue;
           *reinterpret_cast<vec4 *>(dkg + db * 32 + i4 * 8 + g * 4) = a;
           *reinterpret_cast<vec4 *>(dvg + db * 32 + i4 * 8 + g * 4) = b;
         }
@@ -848,12 +853,44 @@ hipError_t launch_group_sum(const Params &p, const GroupSplit &s, int row, int d
   return e;
 }
 
+// A flash_attn_sink_bwd call whose head_dim has no tuned kernel but fits one's columns: dQ from the
+// generic kernel, dK / dV from the tuned one with the columns behind head_dim as zeros (16 heads on
+// 2, 2 x 2048 rows, window 512, d = 96: 67 us against 96 in the generic dK / dV kernel, which holds
+// one wave per SIMD as well and meets two barriers a tile).
+template <typename T, int D>
+static hipError_t launch_bwd_any(const Params &p, int dtype, hipStream_t stream) {
+  if (!p.have_dq && !p.ws_query)
+    if (hipError_t e = launch_dq_any(p, dtype, stream)) return e;
+  Params pk = p;
+  pk.n_nblocks = (p.sk + kKvBlock - 1) / kKvBlock;
+  pk.dk_bs = p.k_bs; pk.dk_rs = p.k_rs; pk.dk_hs = p.k_hs;
+  pk.dv_bs = p.v_bs; pk.dv_rs = p.v_rs; pk.dv_hs = p.v_hs;
+  pk.gsplit = pk.qsplit = 1;
+  const GroupSplit split = plan_group_split(p, (int64_t)pk.n_nblocks * p.b * p.h_k, 256 * (D <= 64 ? 2 : 1), p.d, kQTile, stream);
+  if (p.ws_query) return hipSuccess;  // planning only
+  apply_group_split(pk, p, split, p.d);
+  pk.xcd_remap = idx::block_order_mode(p.b * pk.h_k, p.wr);
+  if (pk.n_nblocks > 0)
+    FA_LAUNCH((dkdv_kernel<T, D, 1, true>), dim3((unsigned)(pk.n_nblocks * p.b * pk.h_k)), dim3(256), stream, pk);
+  hipError_t e = hipGetLastError();
+  if (split.gs * split.qs > 1) {
+    const hipError_t s = launch_group_sum(p, split, p.d, dtype, stream);
+    if (e == hipSuccess) e = s;
+  }
+  return e;
+}
+
 static hipError_t launch_bwd_all(Params &p, int dtype, hipStream_t stream) {
   // The tuned kernels address Q / dO / K / V tiles with 32-bit offsets inside a (batch, head)
   // slice (buffer loads), including a few tiles of look-ahead past the end: larger slices
   // take the generic kernels.
   const int64_t max_rs = std::max(std::max(p.q_rs, p.o_rs), std::max(p.k_rs, p.v_rs));
   const int64_t span = idx::bwd_stream_span_bytes(std::max(p.sq, p.sk), max_rs);
+  if (p.sink && p.d != 32 && p.d != 64 && p.d < 128 && span < (int64_t(1) << 31)) {
+    if (p.d < 32) return dtype == 1 ? launch_bwd_any<_Float16, 32>(p, dtype, stream) : launch_bwd_any<__bf16, 32>(p, dtype, stream);
+    if (p.d < 64) return dtype == 1 ? launch_bwd_any<_Float16, 64>(p, dtype, stream) : launch_bwd_any<__bf16, 64>(p, dtype, stream);
+    return dtype == 1 ? launch_bwd_any<_Float16, 128>(p, dtype, stream) : launch_bwd_any<__bf16, 128>(p, dtype, stream);
+  }
   if (p.drop || (p.d != 32 && p.d != 64 && p.d != 128) || span >= (int64_t(1) << 31)) return launch_bwd_anyd(p, dtype, stream);
   return dtype == 1 ? launch_bwd_t<_Float16>(p, stream) : launch_bwd_t<__bf16>(p, stream);
 }

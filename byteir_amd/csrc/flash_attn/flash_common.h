@@ -242,6 +242,7 @@ hipError_t launch_fwd_anyd(Params &p, int dtype, hipStream_t stream);
 hipError_t launch_bwd_anyd(Params &p, int dtype, hipStream_t stream);
 hipError_t launch_dq_anyd128(const Params &p, int dtype, hipStream_t stream);
 hipError_t launch_dq_exact(const Params &p, int dtype, hipStream_t stream);
+hipError_t launch_dq_any(const Params &p, int dtype, hipStream_t stream);
 
 // Grouped heads with few key blocks (one or two sequences per GPU): a dK/dV workgroup per
 // key/value head and key block leaves most CUs idle, so the query heads of a group are shared

@@ -31,12 +31,12 @@ struct SinkArgs {
 
 // D is head_dim rounded up to 32, 64, 96, 128, 192 or 256; columns from head_dim on are zeros
 template <typename T, int D>
-__global__ void __launch_bounds__(kSinkWaves * 64, D <= 64 ? 2 : 1) sink_dkdv_kernel(const Params p, const SinkArgs a) {
+__global__ void __launch_bounds__(kSinkWaves * 64, D <= 128 ? 2 : 1) sink_dkdv_kernel(const Params p, const SinkArgs a) {
   using vec8 = typename Traits<T>::vec8;
   constexpr int QS = Pad<D>::kPlain;               // row stride of the Q and dO tiles, read plainly and transposed
   constexpr int CPR = D / 8, RPP = 64 / CPR;       // 16-byte chunks per row, rows per pass of a wave
   constexpr int NP = (kSinkRows + RPP - 1) / RPP;
-  constexpr bool kPrefetch = D <= 128;             // the wide tiles leave no registers to hold the next item
+  constexpr bool kPrefetch = D <= 64;              // wider tiles leave no registers to hold the next item: two waves per SIMD cover for each other
   constexpr int kTile = kSinkRows * QS;
   constexpr int RS = D + 4;                        // row stride of the fp32 sums
   static_assert(kSinkKeys * RS * 4 <= 2 * kTile * (int)sizeof(T), "a wave's sums must fit its tiles");
