@@ -31,12 +31,14 @@ struct SinkArgs {
 
 // D is head_dim rounded up to 32, 64, 96, 128, 192 or 256; columns from head_dim on are zeros
 template <typename T, int D>
-__global__ void __launch_bounds__(kSinkWaves * 64, D <= 128 ? 2 : 1) sink_dkdv_kernel(const Params p, const SinkArgs a) {
+__global__ void __launch_bounds__(kSinkWaves * 64, D <= 96 ? 2 : 1) sink_dkdv_kernel(const Params p, const SinkArgs a) {
   using vec8 = typename Traits<T>::vec8;
   constexpr int QS = Pad<D>::kPlain;               // row stride of the Q and dO tiles, read plainly and transposed
   constexpr int CPR = D / 8, RPP = 64 / CPR;       // 16-byte chunks per row, rows per pass of a wave
   constexpr int NP = (kSinkRows + RPP - 1) / RPP;
-  constexpr bool kPrefetch = D <= 64;              // wider tiles leave no registers to hold the next item: two waves per SIMD cover for each other
+  // Two waves per SIMD up to 96 columns; the next item in flight where the registers hold it (at 96 they do
+  // not, and the other wave covers; at 128 they do with one wave, which is as fast as two that spill)
+  constexpr bool kPrefetch = D <= 64 || D == 128;
   constexpr int kTile = kSinkRows * QS;
   constexpr int RS = D + 4;                        // row stride of the fp32 sums
   static_assert(kSinkKeys * RS * 4 <= 2 * kTile * (int)sizeof(T), "a wave's sums must fit its tiles");
@@ -73,36 +75,44 @@ __global__ void __launch_bounds__(kSinkWaves * 64, D <= 128 ? 2 : 1) sink_dkdv_k
   const int i1 = min(items, (share + 1) * per);
 
   T *Qt = tiles[wave], *dOt = tiles[wave] + kTile;
-  uint4 qr[NP], dor[NP];
+  uint4 qr[NP], dor[kPrefetch ? NP : 1];
   float lse_r = INFINITY, dsm_r = 0.f;
   const int ld_c = lane % CPR, ld_r = lane / CPR;
-  auto load_item = [&](int it) {
-    const int hi = hk * group + it / nu, q0 = (u0 + it % nu) * kSinkRows;
-    const T *qg = static_cast<const T *>(p.q) + bi * p.q_bs + hi * p.q_hs + ld_c * 8;
-    const T *dog = static_cast<const T *>(p.dout) + bi * p.o_bs + hi * p.o_hs + ld_c * 8;
+  auto load_rows = [&](const T *rows, int64_t stride, int q0, uint4 *reg) {
 #pragma unroll
     for (int s = 0; s < NP; ++s) {
       const int r = s * RPP + ld_r, q = q0 + r;
-      if (ld_r < RPP && r < kSinkRows && q < p.sq && ld_c * 8 < p.d) {
-        qr[s] = *reinterpret_cast<const uint4 *>(qg + (int64_t)q * p.q_rs);
-        dor[s] = *reinterpret_cast<const uint4 *>(dog + (int64_t)q * p.o_rs);
-      } else {
-        qr[s] = uint4{0, 0, 0, 0};
-        dor[s] = uint4{0, 0, 0, 0};
-      }
+      const bool in = ld_r < RPP && r < kSinkRows && q < p.sq && ld_c * 8 < p.d;
+      reg[s] = in ? *reinterpret_cast<const uint4 *>(rows + (int64_t)q * stride + ld_c * 8) : uint4{0, 0, 0, 0};
     }
-    const int q = q0 + r32;  // +inf: a row that does not exist contributes P = 0
-    lse_r = q < p.sq ? p.lse[((int64_t)bi * p.h + hi) * p.sq + q] * kLog2e : INFINITY;
-    dsm_r = q < p.sq ? p.dsoftmax[((int64_t)bi * p.h + hi) * p.sq_rounded + q] : 0.f;
   };
-  auto store_item = [&]() {
+  auto store_rows = [&](T *tile, const uint4 *reg) {
 #pragma unroll
     for (int s = 0; s < NP; ++s) {
       const int r = s * RPP + ld_r;
-      if (ld_r < RPP && r < kSinkRows) {
-        *reinterpret_cast<uint4 *>(&Qt[r * QS + ld_c * 8]) = qr[s];
-        *reinterpret_cast<uint4 *>(&dOt[r * QS + ld_c * 8]) = dor[s];
-      }
+      if (ld_r < RPP && r < kSinkRows) *reinterpret_cast<uint4 *>(&tile[r * QS + ld_c * 8]) = reg[s];
+    }
+  };
+  auto load_item = [&](int it) {
+    const int hi = hk * group + it / nu, q0 = (u0 + it % nu) * kSinkRows, q = q0 + r32;
+    load_rows(static_cast<const T *>(p.q) + bi * p.q_bs + hi * p.q_hs, p.q_rs, q0, qr);
+    // +inf: a row that does not exist contributes P = 0
+    lse_r = q < p.sq ? p.lse[((int64_t)bi * p.h + hi) * p.sq + q] * kLog2e : INFINITY;
+    dsm_r = q < p.sq ? p.dsoftmax[((int64_t)bi * p.h + hi) * p.sq_rounded + q] : 0.f;
+    const T *dog = static_cast<const T *>(p.dout) + bi * p.o_bs + hi * p.o_hs;
+    if constexpr (kPrefetch) {
+      load_rows(dog, p.o_rs, q0, dor);
+    } else {  // Q, then dO through the same registers
+      store_rows(Qt, qr);
+      load_rows(dog, p.o_rs, q0, qr);
+    }
+  };
+  auto store_item = [&]() {
+    if constexpr (kPrefetch) {
+      store_rows(Qt, qr);
+      store_rows(dOt, dor);
+    } else {
+      store_rows(dOt, qr);
     }
     if (g == 0) { lse_s[wave][r32] = lse_r; dsm_s[wave][r32] = -dsm_r; }
     FA_WAVE_SYNC();  // the wave's own tiles: written by all its lanes, read across lanes
