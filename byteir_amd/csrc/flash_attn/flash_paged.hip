@@ -16,6 +16,9 @@
 // shares its units out evenly over the splits the grid offers it), so a short sequence in a long
 // cache does not wait for one workgroup; rows that nobody sees (outside the window, behind the
 // last key, on an absent page) are not read and count as zeros.
+// Measured, 32 heads on 8, D = 128, fp16: 64 x 8192 keys 340 us = 6.3 TB/s; 64 x 1000..8191 keys
+// (bf16, 1.21 GB) 201 us = 6.0 TB/s; one sequence of 31 keys 8.6 us, of 300 12 us (latency: length,
+// table, rows, then 2 us a unit); 16 heads, D = 64, 64 x 8192 keys 366 us = 5.9 TB/s.
 #include <algorithm>
 
 #include "flash_paged.h"

@@ -13,6 +13,9 @@
 // 4 d bytes a row against 128 d flops a row and key block of MFMA.  The waves' sums meet in LDS,
 // the shares' as fp32 partials that sink_join_kernel adds in order: no atomics, same bits every run.
 // Without scratch there is one share and the workgroup rounds its sums itself.
+// Measured: 4 sinks, 8192 rows, 32 heads on 8, D = 128: 46-50 us (Q and dO, 134 MB, in 20 at the
+// rate of a read stream; four items a wave, each a memory latency); 128 sinks, 2 x 2048 rows, 16
+// heads on 2, d = 96: 26 us.  Two waves per SIMD instead of one with the next item in flight: 38 -> 25 us there.
 #include <algorithm>
 
 #include "flash_common.h"

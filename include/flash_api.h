@@ -32,7 +32,8 @@
  * Calls with few query rows or few query blocks against many keys split the key axis over
  * workgroups and keep their partial results in a stream-ordered allocation
  * (hipMallocAsync / hipFreeAsync on `stream`); the backward call does so for partial dK / dV on
- * small grids when dq_accum cannot hold them; no other call allocates.
+ * small grids when dq_accum cannot hold them, and the bounded-cache calls below do so for theirs
+ * (the weights' scores included); no other call allocates.
  */
 #ifndef BYTEIR_AMD_FLASH_API_H_
 #define BYTEIR_AMD_FLASH_API_H_
