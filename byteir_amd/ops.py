@@ -8,6 +8,7 @@ reference's op kernels: reductions take the canonical [A, B, C] view computed by
 import collections
 import ctypes
 import functools
+import operator
 import struct
 
 import torch
@@ -289,6 +290,17 @@ _PLANS = 4096  # plans kept; serving sees one per batch shape, training one per 
 _Sig = collections.namedtuple("_Sig", "shape stride dtype device")
 
 
+def _nums(scale, *ints):
+    """The scalars of a call as Python numbers: a plan is memoised on their values, and a 0-d tensor in their
+    place would be memoised by its identity."""
+    return float(scale), *map(operator.index, ints)
+
+
+def _window(window):
+    left, right = window
+    return operator.index(left), operator.index(right)
+
+
 def _sig(t):
     return None if t is None else (t.shape, t.stride(), t.dtype, t.get_device())
 
@@ -448,7 +460,8 @@ def flash_attn_sink_fwd(q, k, v, scale, window=(-1, 0), n_sink=0, out=None, work
     flash_attn_workspace_bytes("sink_fwd", ...) bytes; stream: runs there, not on the current stream
     (these three are keywords of the calls below too)."""
     o, lse = out if out is not None else (None, None)
-    plan = _plan_sink_fwd(_sig(q), _sig(k), _sig(v), _sig(o), _sig(lse), scale, tuple(window), n_sink)
+    scale, n_sink = _nums(scale, n_sink)
+    plan = _plan_sink_fwd(_sig(q), _sig(k), _sig(v), _sig(o), _sig(lse), scale, _window(window), n_sink)
     if out is None:
         b, sq, h, _ = q.shape
         o, lse = torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty((b, h, sq), dtype=torch.float32, device=q.device)
@@ -490,7 +503,8 @@ def flash_attn_sink_bwd(dout, q, k, v, o, lse, scale, window=(-1, 0), n_sink=0, 
     are the forward call's.  out: optional (dq, dk, dv, d_softmax, dq_accum, _) of
     flash_attn_bwd_buffers; without it the partial sums of grouped heads go into the workspace."""
     dq, dk, dv, dsm, dq_accum, _ = out if out is not None else (None,) * 6
-    key = (_sig(lse), _sig(dq), _sig(dk), _sig(dv), _sig(dsm), _sig(dq_accum), scale, tuple(window), n_sink)
+    scale, n_sink = _nums(scale, n_sink)
+    key = (_sig(lse), _sig(dq), _sig(dk), _sig(dv), _sig(dsm), _sig(dq_accum), scale, _window(window), n_sink)
     plan = _plan_sink_bwd(_sig(dout), _sig(q), _sig(k), _sig(v), _sig(o), *key)
     if plan is None:
         # the library addresses dout with the strides of o, and the gradients with those of q, k, v
@@ -589,8 +603,9 @@ def flash_attn_paged(q, k_pages, v_pages, block_table, seqlens_k, scale, window=
     the cache after the call; the others are left as they were.
     -> (o, lse[b, h, sq] f32), and weights_out when given."""
     o, lse = out if out is not None else (None, None)
+    scale, n_sink = _nums(scale, n_sink)
     plan = _plan_paged(_sig(q), _sig(k_pages), _sig(v_pages), _sig(block_table), _sig(seqlens_k), _sig(k_new), _sig(v_new), _sig(weights),
-                       _sig(weights_out), _sig(o), _sig(lse), scale, tuple(window), n_sink)
+                       _sig(weights_out), _sig(o), _sig(lse), scale, _window(window), n_sink)
     if out is None:
         b, sq, h, _ = q.shape
         o, lse = torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty((b, h, sq), dtype=torch.float32, device=q.device)
@@ -653,10 +668,11 @@ def flash_attn_evict(k, v, weights, seqlens_k, budget, n_sink=0, n_recent=0, blo
     Without k_out / v_out the cache, weights and seqlens_k are updated IN PLACE; with them (pages with
     out_table, or dense) the rows that stay are copied there and the cache is left alone.  A sequence of
     at most `budget` rows keeps them all; a negative length stays.  Rows, weights behind the last kept
-    one and rows of absent pages are left as they were.
+    one and rows of absent pages are left as they were.  A page that rows move to must appear once, in one
+    sequence's table: pages that sequences share (a common prefix) are cut into another cache.
     -> (kept int32 [b, h_k, budget]: the row each came from, -1 behind the last; weights_out; seqlens_out)."""
     plan = _plan_evict(_sig(k), _sig(v), _sig(weights), _sig(seqlens_k), _sig(block_table), _sig(k_out), _sig(v_out), _sig(out_table),
-                       _sig(weights_out), _sig(seqlens_out), _sig(kept), budget, n_sink, n_recent)
+                       _sig(weights_out), _sig(seqlens_out), _sig(kept), *map(operator.index, (budget, n_sink, n_recent)))
     in_place = k_out is None
     b, hk = seqlens_k.shape[0], k.shape[2]
     if in_place:

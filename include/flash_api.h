@@ -131,7 +131,8 @@ void run_flash_attn_paged_bf16(void **tensors, void *extra_args, void *stream);
  *   -1 behind the last; seqlens_out[i] = min(seqlens_k[i], budget), a negative length stays.
  * In place: k_out = k, v_out = v under the same strides and table (weights_out may then be weights, and
  * seqlens_out may be seqlens_k); otherwise the output cache must not overlap the cache.  Rows and
- * weights behind the last kept row, and rows of absent pages, are left as they were.
+ * weights behind the last kept row, and rows of absent pages, are left as they were.  A page that
+ * rows move to must appear once (of its table, in place): shared pages are cut into another cache.
  * extra_args (192 bytes): i64 k,v,k_out,v_out page_stride; the four row_strides; the four
  * head_strides; b, h_k, d; num_pages, page_size, max_pages of the cache; the same three of the
  * output cache; budget, n_sink, n_recent. */

@@ -381,3 +381,24 @@ def test_a_run_of_them_prompt_evict_decode():
         R.close(w, want["weights"], want["weights_tol"], "weights")
         assert torch.equal(kp, want["k_pages"]) and torch.equal(vp, want["v_pages"])
         n += 1
+
+
+def test_scalars_in_tensors_are_read_at_every_call():
+    """A 0-d tensor as the scale or a count that changes between calls: each call takes its value then."""
+    g = gen(5)
+    q, k, v = randn(g, 1, 40, 2, 64), randn(g, 1, 90, 2, 64), randn(g, 1, 90, 2, 64)
+    scale, sinks, left = torch.tensor(0.0625), torch.tensor(0), torch.tensor(7)
+    lens = torch.tensor([90], dtype=torch.int32, device="cuda")
+    w = torch.rand(1, 2, 90, generator=g, device="cuda")
+    for s, n, wl in ((0.0625, 0, 7), (0.25, 3, 7), (0.25, 3, 20)):
+        scale.fill_(s), sinks.fill_(n), left.fill_(wl)
+        o, lse = ops.flash_attn_sink_fwd(q, k, v, scale, (left, 0), sinks)
+        want = ops.flash_attn_sink_fwd(q, k, v, s, (wl, 0), n)
+        assert torch.equal(o, want[0]) and torch.equal(lse, want[1])
+        grads = ops.flash_attn_sink_bwd(q, q, k, v, o, lse, scale, (left, 0), sinks)
+        assert all(map(torch.equal, grads, ops.flash_attn_sink_bwd(q, q, k, v, o, lse, s, (wl, 0), n)))
+        got = ops.flash_attn_paged(q[:, :2], k, v, None, lens, scale, (left, 0), sinks)
+        assert all(map(torch.equal, got, ops.flash_attn_paged(q[:, :2], k, v, None, lens, s, (wl, 0), n)))
+        got = ops.flash_attn_evict(k, v, w, lens, left, sinks, k_out=torch.zeros_like(k), v_out=torch.zeros_like(v))
+        want = ops.flash_attn_evict(k, v, w, lens, wl, n, k_out=torch.zeros_like(k), v_out=torch.zeros_like(v))
+        assert all(map(torch.equal, got, want))
