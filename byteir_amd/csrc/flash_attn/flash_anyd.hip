@@ -389,7 +389,7 @@ __global__ void __launch_bounds__(256) dot_do_o_anyd_kernel(const Params p) {
 #pragma unroll
   for (int m = 16; m > 0; m >>= 1) s += __shfl_xor(s, m, 64);
   if (p.drop) s *= p.p_keep;  // flash_bwd_preprocess_kernel.h:124-128
-  if (ok && sub == 0) p.dsoftmax[((int64_t)bi * p.h + hi) * p.sq_rounded + i] = s;
+  if (ok && sub == 0 && i >= p.d_rows) p.dsoftmax[((int64_t)bi * p.h + hi) * p.sq_rounded + i] = s;
 }
 
 // ---- backward 2: dK, dV -----------------------------------------------------------------------------
@@ -566,7 +566,7 @@ __global__ void __launch_bounds__(256, DR <= 64 ? 2 : 1) dkdv_anyd_kernel(const 
 // Exact: D = dO . O, which the kernel takes from the stored O itself, carries the roundings of that O (its
 // own and those of P in P V).  With e = sum_j P (dP - D), which would be zero for the D of these P
 // and dP, D + e has none of them; dQ is corrected by -e scale sum_j P K (one more product that shares
-// the K fragments of dS K), and D + e is written for the dK / dV kernel.
+// the K fragments of dS K), and D + e is written for the dK / dV kernel.  With d_rows only D + e is wanted.
 template <typename T, int DR, bool Drop, bool Sink = false, bool Exact = false>
 __global__ void __launch_bounds__(256, (Exact ? DR <= 64 : DR <= 96 || (DR == 128 && !Drop)) ? 2 : 1) dq_anyd_kernel(const Params p) {
   using vec8 = typename Traits<T>::vec8;
@@ -623,6 +623,7 @@ __global__ void __launch_bounds__(256, (Exact ? DR <= 64 : DR <= 96 || (DR == 12
     }
     dsm_l += partner32(dsm_l);  // the other half of the columns
   }
+  const bool d_only = Exact && p.d_rows > 0;
   float err = 0.f;                             // Exact: this lane's part of e
   float16v dq_acc[DR / 32], pk_acc[Exact ? DR / 32 : 1];
 #pragma unroll
@@ -697,6 +698,7 @@ __global__ void __launch_bounds__(256, (Exact ? DR <= 64 : DR <= 96 || (DR == 12
       }
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
+        if (d_only) break;
         float f[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) f[j] = s[w >> 1][(w & 1) * 8 + j];
@@ -725,6 +727,7 @@ __global__ void __launch_bounds__(256, (Exact ? DR <= 64 : DR <= 96 || (DR == 12
   if constexpr (Exact) {
     err += partner32(err);  // the other half of the keys
     if (qrow < p.sq && g == 0) p.dsoftmax[((int64_t)bi * p.h + hi) * p.sq_rounded + qrow] = dsm_l + err;
+    if (d_only) return;
 #pragma unroll
     for (int db = 0; db < DR / 32; ++db)
 #pragma unroll
@@ -781,12 +784,13 @@ hipError_t fwd_anyd_d(Params &p, hipStream_t stream) {
   return hipGetLastError();
 }
 
+// the blocks of a call's first n_rows rows
 template <typename T, int DR, bool Exact>
-hipError_t dq_sink_d(const Params &p, hipStream_t stream) {
+hipError_t dq_sink_d(const Params &p, int n_rows, hipStream_t stream) {
   Params pq = p;
   pq.pack = head_pack(p, 4);
   const int n_heads = p.h >> pq.pack, rows = kRows >> pq.pack;
-  pq.n_mblocks = (p.sq + rows - 1) / rows;
+  pq.n_mblocks = (n_rows + rows - 1) / rows;
   if (pq.n_mblocks == 0) return hipSuccess;
   pq.xcd_remap = idx::block_order_mode(p.b * n_heads, p.wr);
   FA_LAUNCH((dq_anyd_kernel<T, DR, false, true, Exact>), dim3((unsigned)(pq.n_mblocks * p.b * n_heads)), dim3(256), stream, pq);
@@ -814,7 +818,7 @@ hipError_t bwd_anyd_d(const Params &p, hipStream_t stream) {
     }
   }
   if (p.n_mblocks > 0 && !p.ws_query && !p.have_dq) {
-    if (p.sink) return dq_sink_d<T, DR, false>(p, stream);
+    if (p.sink) return dq_sink_d<T, DR, false>(p, p.sq, stream);
     if (p.drop) FA_LAUNCH((dq_anyd_kernel<T, DR, true>), gq, block, stream, p);
     else FA_LAUNCH((dq_anyd_kernel<T, DR, false>), gq, block, stream, p);
   }
@@ -861,20 +865,20 @@ hipError_t launch_dq_anyd128(const Params &p, int dtype, hipStream_t stream) {
   pq.n_mblocks = (p.sq + kRows - 1) / kRows;
   if (pq.n_mblocks == 0) return hipSuccess;
   const dim3 grid((unsigned)(pq.n_mblocks * p.b * p.h)), block(256);
-  if (p.sink) return dtype == 1 ? dq_sink_d<_Float16, 128, false>(p, stream) : dq_sink_d<__bf16, 128, false>(p, stream);
+  if (p.sink) return dtype == 1 ? dq_sink_d<_Float16, 128, false>(p, p.sq, stream) : dq_sink_d<__bf16, 128, false>(p, p.sq, stream);
   if (dtype == 1) FA_LAUNCH((dq_anyd_kernel<_Float16, 128, false>), grid, block, stream, pq);
   else FA_LAUNCH((dq_anyd_kernel<__bf16, 128, false>), grid, block, stream, pq);
   return hipGetLastError();
 }
 
 template <typename T, bool Exact>
-hipError_t dq_sink_t(const Params &p, hipStream_t stream) {
-  if (p.d <= 32) return dq_sink_d<T, 32, Exact>(p, stream);
-  if (p.d <= 64) return dq_sink_d<T, 64, Exact>(p, stream);
-  if (p.d <= 96) return dq_sink_d<T, 96, Exact>(p, stream);
-  if (p.d <= 128) return dq_sink_d<T, 128, Exact>(p, stream);
-  if (p.d <= 192) return dq_sink_d<T, 192, Exact>(p, stream);
-  return dq_sink_d<T, 256, Exact>(p, stream);
+hipError_t dq_sink_t(const Params &p, int n_rows, hipStream_t stream) {
+  if (p.d <= 32) return dq_sink_d<T, 32, Exact>(p, n_rows, stream);
+  if (p.d <= 64) return dq_sink_d<T, 64, Exact>(p, n_rows, stream);
+  if (p.d <= 96) return dq_sink_d<T, 96, Exact>(p, n_rows, stream);
+  if (p.d <= 128) return dq_sink_d<T, 128, Exact>(p, n_rows, stream);
+  if (p.d <= 192) return dq_sink_d<T, 192, Exact>(p, n_rows, stream);
+  return dq_sink_d<T, 256, Exact>(p, n_rows, stream);
 }
 
 // D and dQ of a flash_attn_sink_bwd call, every head_dim
@@ -885,12 +889,13 @@ hipError_t launch_dq_any(const Params &p, int dtype, hipStream_t stream) {
   if (dtype == 1) FA_LAUNCH((dot_do_o_anyd_kernel<_Float16>), grid, dim3(256), stream, p);
   else FA_LAUNCH((dot_do_o_anyd_kernel<__bf16>), grid, dim3(256), stream, p);
   if (hipError_t e = hipGetLastError()) return e;
-  return dtype == 1 ? dq_sink_t<_Float16, false>(p, stream) : dq_sink_t<__bf16, false>(p, stream);
+  return dtype == 1 ? dq_sink_t<_Float16, false>(p, p.sq, stream) : dq_sink_t<__bf16, false>(p, p.sq, stream);
 }
 
-// dQ and D of a flash_attn_sink_bwd call without the roundings that D takes from the stored O
-hipError_t launch_dq_exact(const Params &p, int dtype, hipStream_t stream) {
-  return dtype == 1 ? dq_sink_t<_Float16, true>(p, stream) : dq_sink_t<__bf16, true>(p, stream);
+// dQ and D of the first n_rows rows of a flash_attn_sink_bwd call without the roundings that D takes from
+// the stored O; with d_rows D alone
+hipError_t launch_dq_exact(const Params &p, int dtype, int n_rows, hipStream_t stream) {
+  return dtype == 1 ? dq_sink_t<_Float16, true>(p, n_rows, stream) : dq_sink_t<__bf16, true>(p, n_rows, stream);
 }
 
 hipError_t launch_bwd_anyd(Params &p, int dtype, hipStream_t stream) {

@@ -45,7 +45,7 @@ __global__ void __launch_bounds__(256) dot_do_o_kernel(const Params p) {
   for (int j = 0; j < 8; ++j) s += (float)a[j] * (float)o[j];
 #pragma unroll
   for (int m = LPR / 2; m > 0; m >>= 1) s += __shfl_xor(s, m, 64);
-  if (ok && sub == 0) p.dsoftmax[((int64_t)bi * p.h + hi) * p.sq_rounded + i] = s;
+  if (ok && sub == 0 && i >= p.d_rows) p.dsoftmax[((int64_t)bi * p.h + hi) * p.sq_rounded + i] = s;
 }
 
 constexpr int kKvBlock = 128;  // keys per workgroup in dkdv (32 per wave)
@@ -919,8 +919,15 @@ hipError_t launch_bwd(Params &p, int dtype, hipStream_t stream) {
   // 1.50 roundings rms against 64 bits with D as it is, 1.42 so).
   const int64_t seen = p.wl < 0 || p.wr < 0 ? p.sk : std::min<int64_t>(p.sk, (int64_t)p.wl + p.wr + 1 + p.n_sink);
   if (seen <= 512) {
-    if (hipError_t e = launch_dq_exact(p, dtype, stream)) return e;
+    if (hipError_t e = launch_dq_exact(p, dtype, p.sq, stream)) return e;
     p.have_dq = 1;
+  } else if (p.wr >= 0) {
+    // elsewhere the first rows of a causal call, which see at most 64 keys, hold nearly all of that
+    // error (their dQ and their share of dK are also the largest): they take their D from that kernel
+    // (dQ and dK off by up to 1.6 roundings rms before, 1.42-1.49 so; 10-14 us of 196 and 1465)
+    const int64_t few = std::min<int64_t>(p.sq, 64 - ((int64_t)p.sk - p.sq) - p.wr);
+    p.d_rows = few > 0 ? (int)few : 0;
+    if (hipError_t e = launch_dq_exact(p, dtype, p.d_rows, stream)) return e;
   }
   if (hipError_t e = launch_bwd_all(p, dtype, stream)) return e;
   const bool rest = p.ws && p.ws_bytes > base;

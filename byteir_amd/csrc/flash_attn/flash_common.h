@@ -195,6 +195,7 @@ struct Params {
   int pack;                           // with sinks: log2 of the query heads that share a workgroup
   int n_sink;                         // the first n_sink keys stay visible outside the window
   int have_dq;                        // backward: 1: dq and dsoftmax have been written (launch_dq_exact)
+  int d_rows;                         // backward: rows [0, d_rows) of every head have their dsoftmax (launch_dq_exact)
   int kv_lo, kv_hi;                   // backward: the keys that some query row can see (dK/dV kernels load no others)
   int n_mblocks, n_nblocks;
   int xcd_remap;                      // 0: by (batch, head); 1: blocks of a (batch, head) share an XCD; 2: 1 + longest blocks of all heads first; 3: longest first without XCD grouping
@@ -241,7 +242,7 @@ __device__ __forceinline__ void row_limits(const Params &p, int q, int &lo, int 
 hipError_t launch_fwd_anyd(Params &p, int dtype, hipStream_t stream);
 hipError_t launch_bwd_anyd(Params &p, int dtype, hipStream_t stream);
 hipError_t launch_dq_anyd128(const Params &p, int dtype, hipStream_t stream);
-hipError_t launch_dq_exact(const Params &p, int dtype, hipStream_t stream);
+hipError_t launch_dq_exact(const Params &p, int dtype, int n_rows, hipStream_t stream);
 hipError_t launch_dq_any(const Params &p, int dtype, hipStream_t stream);
 
 // Grouped heads with few key blocks (one or two sequences per GPU): a dK/dV workgroup per

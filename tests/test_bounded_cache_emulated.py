@@ -33,6 +33,8 @@ SINK_CASES = [
     (1, 150, 150, 1, 1, 64, (0, 0), 2),        # a window of the row's own key
     (1, 100, 260, 2, 2, 40, (-1, 0), 4),       # no left side: sinks change nothing
     (1, 64, 200, 1, 1, 64, (25, -1), 300),     # no right side, sinks beyond the keys
+    (1, 520, 520, 1, 1, 64, (600, 0), 4),      # rows of more than 512 keys: D of the first rows in a launch of its own
+    (1, 516, 530, 1, 1, 40, (550, 2), 0),      # the same, columns behind head_dim
     (1, 140, 140, 2, 1, 256, (33, 0), 5),      # the widest head
     (1, 200, 0, 1, 1, 64, (9, 0), 4),          # no keys
 ]

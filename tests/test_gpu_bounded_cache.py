@@ -402,3 +402,27 @@ def test_scalars_in_tensors_are_read_at_every_call():
         got = ops.flash_attn_evict(k, v, w, lens, left, sinks, k_out=torch.zeros_like(k), v_out=torch.zeros_like(v))
         want = ops.flash_attn_evict(k, v, w, lens, wl, n, k_out=torch.zeros_like(k), v_out=torch.zeros_like(v))
         assert all(map(torch.equal, got, want))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("s, ahead, h, hk, d", [(300, 0, 2, 2, 64), (900, 0, 4, 2, 64), (900, 0, 2, 1, 128), (700, 40, 3, 3, 72), (600, 0, 2, 2, 192),
+                                                (2500, 0, 16, 16, 128)])
+def test_rows_of_few_keys_have_no_rounding_of_the_stored_output(s, ahead, h, hk, d, dtype):
+    """The first row of a causal call, which sees one key, has dS = dP - D = 0.  With D from the stored O, dS would be
+    off by the rounding of that O, half a step of the type; without it three dot products of d terms in fp32 are
+    left (dP of either kernel, D), each off by (d + 2) 2^-24 sum |dO V|, one rounding of D, and what P is off
+    times that rounding of O, far below another.  dS is then rounded to the type's least step."""
+    g = gen(s + d)
+    q, k, v, do = (randn(g, 1, s, n, d, dtype=dtype) for n in (h, hk, hk, h))
+    q, do = q[:, ahead:], do[:, ahead:]
+    if ahead:  # row 0 sees ahead + 1 keys: all but one far below it
+        k[:, :ahead], q[:, 0], k[:, ahead] = -8.0, 8.0, 8.0
+    scale = 1 / math.sqrt(d)
+    o, lse = ops.flash_attn_sink_fwd(q, k, v, scale, (s, 0), 4)
+    dq, _, _ = ops.flash_attn_sink_bwd(do, q, k, v, o, lse, scale, (s, 0), 4)
+    grow = lambda t: t[0, ahead].double().abs().repeat_interleave(h // hk, 0)
+    dp = (do[0, 0].double().abs() * grow(v)).sum(1, keepdim=True)
+    tol = scale * grow(k) * (4 * (d + 2) * 2.0 ** -24 * dp + R.half_step(dtype) * R.LEAST[R.half_step(dtype)])
+    if dtype == torch.float16:
+        tol = tol + 2.0 ** -25  # the rounding of dq itself
+    R.close(dq[0, 0], torch.zeros_like(tol), tol, (s, h, d, dtype))
