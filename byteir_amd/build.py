@@ -8,6 +8,9 @@ Targets:
   flash   -> lib/libflash_attn.so         flash-attention custom library (C ABI)
   brt     -> lib/libbrt.so                BRT-shaped C++ host runtime (g++, no HIP headers)
   index_check -> lib/libfa_index_check.so host-only bounds check of the flash-attention index arithmetic
+and, for the tests alone (a build of everything goes on without one that fails):
+  test_kernels -> tests/external_kernels/libcustom_add.so
+  emu -> tests/emu/lib/*.so               the same sources for the host
 """
 import os
 import subprocess
@@ -89,7 +92,8 @@ def build_emu(verbose=False):
     clang against tests/emu/wave_emu.h (which stands in for the HIP runtime header and runs every
     lane as a fiber), a host stand-in for the device layer, and the runtime linked against them
     -- tests/emu/lib/{libbrt_rocm_kernels,libflash_attn,libbrt}.so, the same C ABIs on host
-    memory, for the tests that need no GPU.  Needs a host clang (vector extensions, _Float16,
+    memory, for the tests that need no GPU.  What the sources need of that header changes no
+    more: later additions to it are made beside the sources (FA_EMULATE in flash_common.h).  Needs a host clang (vector extensions, _Float16,
     __bf16); skipped when there is none.  Nothing in the package loads these."""
     clang = os.path.join(os.environ.get("ROCM_PATH", "/opt/rocm"), "llvm", "bin", "clang++")
     emu = os.path.join(ROOT, "tests", "emu")
@@ -120,13 +124,28 @@ def build_emu(verbose=False):
              + [f"-L{out}", "-lbrt_rocm_kernels", "-ldl", "-Wl,-rpath,$ORIGIN"], verbose)
 
 
+# what only tests load: {target: what it writes}
+TEST_TARGETS = {"test_kernels": ("tests/external_kernels/libcustom_add.so",),
+                "emu": tuple(f"tests/emu/lib/{n}.so" for n in ("libflash_attn", "libbrt_rocm_kernels", "libbrt"))}
 TARGETS = {"kernels": build_kernels, "flash": build_flash, "brt": build_brt, "index_check": build_index_check,
            "test_kernels": build_test_kernels, "emu": build_emu}
 
 
 def build_all(verbose=False, targets=None):
-    for name in targets or ("kernels", "flash", "brt", "index_check", "test_kernels", "emu"):
-        TARGETS[name](verbose)
+    """The named targets, or all.  Of all, those for the tests may fail (a tests/ directory of another age): that is
+    printed, and nothing older is left in their place for a test to load."""
+    for name in targets or TARGETS:
+        old = [os.path.join(ROOT, f) for f in TEST_TARGETS.get(name, ())]
+        for f in filter(os.path.exists, old):
+            os.remove(f)
+        try:
+            TARGETS[name](verbose)
+        except Exception as e:
+            if targets or name not in TEST_TARGETS:
+                raise
+            for f in filter(os.path.exists, old):
+                os.remove(f)
+            print(f"[build] {name} (for the tests only) does not build, going on without it: {e}", file=sys.stderr)
 
 
 if __name__ == "__main__":

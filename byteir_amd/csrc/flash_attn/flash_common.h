@@ -26,8 +26,6 @@
 #ifndef FA_LAUNCH
 #define FA_LAUNCH(kernel, grid, block, stream, ...) kernel<<<(grid), (block), 0, (stream)>>>(__VA_ARGS__)
 #endif
-// Consumes a value in a vector register at this point of the program: the wait for the loads
-// that produce it is placed here instead of in front of its first use.
 // Marks a point where the lanes of one wave exchange data through LDS without a workgroup
 // barrier: what all lanes wrote before it is read by other lanes of the same wave after it.
 // On the GPU a wave executes its LDS instructions in program order for all lanes at once, so
@@ -35,9 +33,21 @@
 #ifndef FA_WAVE_SYNC
 #define FA_WAVE_SYNC() ((void)0)
 #endif
+// Consumes a value in a vector register at this point of the program: the wait for the loads
+// that produce it is placed here instead of in front of its first use.
 #ifndef FA_PIN
 #define FA_PIN(x) asm volatile("" : "+v"(x))
 #define FA_PIN2(x, y) asm volatile("" : "+v"(x), "+v"(y))
+#endif
+// GPU operations that a host build has to replace are replaced here, beside the sources that use them: what
+// such a build brings along (FA_LAUNCH and the like, the builtins behind the MFMA and lane wrappers
+// below) then serves older and newer sources alike.
+#ifdef FA_EMULATE
+#define FA_READLANE(v, lane) __builtin_amdgcn_ds_bpermute((lane) * 4, (v))
+#define FA_LDS_ADD(p, v) ((void)(*(p) += (v)))  // the lanes of a workgroup take turns in one thread
+#else
+#define FA_READLANE(v, lane) __builtin_amdgcn_readlane((v), (lane))  // a scalar
+#define FA_LDS_ADD(p, v) ((void)atomicAdd((p), (v)))
 #endif
 
 namespace fa {

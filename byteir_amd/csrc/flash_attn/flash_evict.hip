@@ -91,7 +91,7 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictPa
     for (int i = tid; i < kBins; i += kSelThreads) hist[i] = 0;
     __syncthreads();
     each([&](int, uint32_t u, bool ok) {
-      if (ok && (u & mask) == prefix) atomicAdd(&hist[(u >> shift) & digit], 1u);
+      if (ok && (u & mask) == prefix) FA_LDS_ADD(&hist[(u >> shift) & digit], 1u);
     });
     __syncthreads();
     // bins from the greatest down, two per thread: rows in the bins above this thread's

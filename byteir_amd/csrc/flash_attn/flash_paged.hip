@@ -134,7 +134,7 @@ __global__ void __launch_bounds__(kWaves * 64, D <= 128 ? 2 : 1) paged_kernel(co
     if (u.staged && scalar_rows) {
 #pragma unroll
       for (int s = 0; s < NPV; ++s) {
-        const int64_t pg = __builtin_amdgcn_readlane(pg_next, s * RPP), row = __builtin_amdgcn_readlane(row_next, s * RPP);
+        const int64_t pg = FA_READLANE(pg_next, s * RPP), row = FA_READLANE(row_next, s * RPP);
         const u32x4 a = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(kg + pg * p.pages.k_ps + row * p.pages.k_rs + k_in));
         const u32x4 b = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(vg + pg * p.pages.v_ps + row * p.pages.v_rs + v_in));
         u.k[s] = uint4{a.x, a.y, a.z, a.w};
@@ -481,9 +481,11 @@ hipError_t paged_td(PagedParams &p, hipStream_t stream) {
   bool owned = false;
   if (need) {
     if (p.ws && (reinterpret_cast<uintptr_t>(p.ws) & 15) == 0 && p.ws_bytes >= need) ws = p.ws;
-    else if (hipMallocAsync(&ws, need, stream) == hipSuccess) owned = true;
-    else { (void)hipGetLastError(); ws = nullptr; }
-    if (!ws && s_bytes) return hipErrorOutOfMemory;  // the scores have nowhere to go
+    else if (const hipError_t e = hipMallocAsync(&ws, need, stream)) {
+      (void)hipGetLastError();
+      if (s_bytes) return e;  // the scores have nowhere to go
+      ws = nullptr;
+    } else owned = true;
     if (!ws) p.n_splits = 1;
     else {
       p.s_part = s_bytes ? static_cast<float *>(ws) : nullptr;
