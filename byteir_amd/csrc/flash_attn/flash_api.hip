@@ -134,10 +134,12 @@ struct Reader {
   float f32() { float v; memcpy(&v, s, 4); s += 4; return v; }
 };
 
-// extra_args of flash_attn_sink_{fwd,bwd}: the forward blob (192 bytes), then n_sink
+// extra_args of flash_attn_sink_{fwd,bwd}: the forward blob (192 bytes), then n_sink.  The windows that end
+// the forward blob are read whole here, like those of flash_attn_paged: parse() cuts them to 32
+// bits, as the forward call does, and 2^32 would be a window of 0.
 int sink_args(const void *extra_args, const Blob &a, fa::Params &p) {
-  Reader r{static_cast<const unsigned char *>(extra_args) + 192};
-  const int64_t n_sink = r.i64();
+  Reader r{static_cast<const unsigned char *>(extra_args) + 176};
+  const int64_t wl = r.i64(), wr = r.i64(), n_sink = r.i64();
   if (n_sink < 0) return fail("n_sink %ld is negative", (long)n_sink);
   if (p.drop) return fail("dropout is not supported with sinks");
   if (!(a.softmax_scale > 0.f) || std::isinf(a.softmax_scale)) return fail("softmax_scale %g is not positive and finite", a.softmax_scale);
@@ -146,8 +148,8 @@ int sink_args(const void *extra_args, const Blob &a, fa::Params &p) {
   p.n_sink = (int)(n_sink < a.seqlen_k ? n_sink : a.seqlen_k);
   // rows, keys and windows are added in 32 bits; a side that reaches past every key is no bound
   if (a.seqlen_q + a.seqlen_k > (1 << 29)) return fail("problem too large for 32-bit tile indices");
-  if (a.window_size_left >= a.seqlen_k) p.wl = -1;
-  if (a.window_size_right >= a.seqlen_q) p.wr = -1;
+  p.wl = wl < 0 || wl >= a.seqlen_k ? -1 : (int)wl;
+  p.wr = wr < 0 || wr >= a.seqlen_q ? -1 : (int)wr;
   return 0;
 }
 

@@ -93,7 +93,8 @@ void run_flash_attn_kvcache_bf16(void **tensors, void *extra_args, void *stream)
  * Attention with a window and sinks, and its gradient.  Row i sees key j when the window's right
  * side admits it (j <= i + seqlen_k - seqlen_q + right) and either its left side does
  * (j >= i + seqlen_k - seqlen_q - left) or j < n_sink.  Tensors as run_flash_attn_fwd / _bwd
- * (rng_state is not read); extra_args (200 bytes): theirs, then i64 n_sink.  p_dropout must be 0,
+ * (rng_state is not read); extra_args (200 bytes): theirs, then i64 n_sink; the windows are read as the
+ * i64 they are, not cut to 32 bits, and one wider than everything is none.  p_dropout must be 0,
  * softmax_scale positive and finite, head_dim a multiple of 8 up to 256.  softmax_lse comes from
  * unrounded fp32 sums at every head_dim; a row that sees no key gives O = 0, LSE = +inf and no
  * gradient; a key that no row of a 256-row block sees is not read there.  dq_accum may be NULL. */
