@@ -346,9 +346,16 @@ int paged_impl(void **tensors, const void *extra_args, int dtype, const Scratch 
   if (h / h_k * sq > (1 << 30) || tiles > (1 << 22) || b * h * sq > (1 << 30) || b * h_k * n_new > (1ll << 31) / (d / 8) || b * h_k * (cap / 256 + 1) > (1 << 23))
     return fail("problem too large for 32-bit tile indices");
   if (sc.query) *sc.query = 0;
-  if (b == 0 || sq == 0) {  // nothing attends; new rows are still appended
-    if (b == 0 || n_new == 0 || sc.query) return 0;
-    return fail("new rows without query rows (seqlen_q 0, seqlen_knew %ld)", (long)n_new);
+  if (b == 0) return 0;
+  if (sq == 0) {  // nothing attends: no key's weight grows, and new rows are refused
+    if (n_new) return sc.query ? 0 : fail("new rows without query rows (seqlen_q 0, seqlen_knew %ld)", (long)n_new);
+    if (!weights || sc.query) return 0;
+    if (max_pages) p.pages.table = static_cast<const int *>(tensors[5]);
+    p.seqlens = static_cast<const int *>(tensors[6]);
+    if (weights == 2) p.w_in = static_cast<const float *>(tensors[9]);
+    p.w_out = static_cast<float *>(tensors[10]);
+    if (!p.seqlens || (max_pages && !p.pages.table) || (weights == 2 && !p.w_in) || !p.w_out) return fail("null tensor pointer");
+    return fa::launch_paged(p, dtype, static_cast<hipStream_t>(stream));
   }
   if (sc.query) {
     static float any;  // only whether there are weights matters when planning

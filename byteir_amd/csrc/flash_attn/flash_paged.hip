@@ -449,6 +449,11 @@ __global__ void __launch_bounds__(256) paged_weights_kernel(const PagedParams p)
     if (y < n) p.w_out[at + y] = w[y];
 }
 
+hipError_t launch_weights(const PagedParams &p, hipStream_t stream) {
+  FA_LAUNCH((paged_weights_kernel), dim3((unsigned)((int64_t)((p.pages.capacity() + 1023) / 1024) * p.b * p.h_k)), dim3(256), stream, p);
+  return hipGetLastError();
+}
+
 // the new rows into the cache, 16 bytes a thread; rows behind the capacity or on an absent page are dropped
 __global__ void __launch_bounds__(256) paged_append_kernel(const PagedParams p) {
   const int cpr = p.d / 8;
@@ -510,10 +515,7 @@ hipError_t paged_td(PagedParams &p, hipStream_t stream) {
   if (e == hipSuccess && p.o_part) {
     e = join_td<T, D>(p, 0, stream);
   }
-  if (e == hipSuccess && p.w_out) {
-    FA_LAUNCH((paged_weights_kernel), dim3((unsigned)((int64_t)((p.pages.capacity() + 1023) / 1024) * p.b * p.h_k)), dim3(256), stream, p);
-    e = hipGetLastError();
-  }
+  if (e == hipSuccess && p.w_out) e = launch_weights(p, stream);
   if (owned) {
     const hipError_t f = hipFreeAsync(ws, stream);
     if (e == hipSuccess) e = f;
@@ -534,6 +536,7 @@ hipError_t paged_t(PagedParams &p, hipStream_t stream) {
 hipError_t launch_paged(PagedParams &p, int dtype, hipStream_t stream) {
   const int cap = p.pages.capacity();
   p.n_ct = (p.h / p.h_k * p.sq + 31) / 32;
+  if (p.sq == 0) return launch_weights(p, stream);  // no columns: weights_out = weights, or zero
   // most units a tile visits: the sinks' and those of a window over its rows, or the whole cache
   int64_t units = (cap + kUnit - 1) / kUnit;
   if (p.wl >= 0)

@@ -600,7 +600,7 @@ def flash_attn_paged(q, k_pages, v_pages, block_table, seqlens_k, scale, window=
     weights / weights_out f32 [b, h_k, capacity] (weights_out may be weights): when weights_out is given,
     weights_out[i, c, j] = weights[i, c, j] (0 without weights, and for rows appended by this call) + the
     attention that key j got from all query rows and heads of key/value head c, for the rows j in
-    the cache after the call; the others are left as they were.
+    the cache after the call; the others are left as they were.  Without query rows (sq 0) new rows are refused.
     -> (o, lse[b, h, sq] f32), and weights_out when given."""
     o, lse = out if out is not None else (None, None)
     scale, n_sink = _nums(scale, n_sink)

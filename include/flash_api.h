@@ -118,6 +118,7 @@ void run_flash_attn_sink_bwd_bf16(void **tensors, void *extra_args, void *stream
  * The weights mode is 0 (neither tensor is touched), 1 (weights_out = the attention each key got
  * from all query rows and heads of its key/value head) or 2 (that on top of `weights`; appended rows
  * start from 0; weights_out may be weights); rows behind the last key are left as they were.
+ * Without query rows (seqlen_q 0) new rows are refused and no weight grows.
  * extra_args (252 bytes): i64 q,k,v,knew,vnew,o batch_stride (of k, v: page stride); the same six
  * row_strides; the same six head_strides; i64 b, h, h_k, d, seqlen_knew; f32 softmax_scale;
  * i64 seqlen_q, num_pages, page_size, max_pages, window_size_left, _right, n_sink, weights mode. */

@@ -1,0 +1,43 @@
+"""The bounded-cache calls at the limits of what they take, on the GPU (the same on the host: test_bounded_cache_limits)."""
+import pytest
+import torch
+
+import bounded_cache_ref as R
+from byteir_amd import ops
+
+pytestmark = pytest.mark.gpu
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def randn(g, *shape, dtype=torch.float16):
+    return torch.randn(shape, generator=g, device="cuda").to(dtype)
+
+
+def test_windows_beyond_32_bits():
+    g = gen(1)
+    q, k, v, do = (randn(g, 1, n, 2, 64) for n in (80, 300, 300, 80))
+    for window, same in (((1 << 32, 0), (-1, 0)), (((1 << 32) + 3, 1 << 32), (-1, -1)), ((9, (1 << 32) + 1), (9, -1))):
+        want, got = (ops.flash_attn_sink_fwd(q, k, v, 0.125, w, 3) for w in (same, window))
+        assert all(map(torch.equal, got, want))
+        grads, other = (ops.flash_attn_sink_bwd(do, q, k, v, *got, 0.125, w, 3) for w in (same, window))
+        assert all(map(torch.equal, grads, other))
+
+
+@pytest.mark.parametrize("paged", [False, True])
+def test_no_query_rows_keep_the_weights(paged):
+    g = gen(2)
+    b, hk, cap = 3, 2, 2100
+    k = randn(g, *((400, 21) if paged else (b, cap)), hk, 64)
+    table = torch.randperm(400, generator=g, device="cuda")[:300].to(torch.int32).view(b, 100).contiguous() if paged else None
+    lens = torch.tensor([1500, -1, cap], dtype=torch.int32, device="cuda")
+    w, out = torch.rand(b, hk, cap, generator=g, device="cuda"), torch.full((b, hk, cap), -7.0, device="cuda")
+    ops.flash_attn_paged(randn(g, b, 0, 4, 64), k, k, table, lens, 0.125, weights=w, weights_out=out)
+    want = torch.full_like(out, -7.0)
+    want[0, :, :1500], want[2] = w[0, :, :1500], w[2]
+    assert torch.equal(out, want)
+    ops.flash_attn_paged(randn(g, b, 0, 4, 64), k, k, table, lens, 0.125, weights_out=out)
+    want[0, :, :1500], want[2] = 0, 0
+    assert torch.equal(out, want)
