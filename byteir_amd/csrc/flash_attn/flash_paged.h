@@ -55,8 +55,13 @@ struct PagedParams {
   int n_ct;                  // tiles of 32 columns (query head of the group x query row)
   int max_units;             // most 32-key units a column tile can visit
   int n_splits, min_units;   // workgroups that share a tile's units, fewest units of one
-  float *o_part, *ml_part;   // [n_splits][b][h][sq][tile width], [n_splits][b][h][sq][2]; null: n_splits == 1
-  float *s_part;             // [b][h_k][group * sq][max_units * 32] scores, for the weights
+  // What one launch computes: column tiles [tile0, tile0 + n_tiles), numbered through (sequence, key/value head,
+  // tile), whose rows ((sequence * h + head) * sq + query row) are [row0, row0 + n_rows).  All of them, unless
+  // the scores of all would take more than kScoreBytes.
+  int tile0, n_tiles;
+  int64_t row0, n_rows;
+  float *o_part, *ml_part;   // [n_splits][n_rows][tile width], [n_splits][n_rows][2]; null: n_splits == 1
+  float *s_part;             // [n_rows][max_units * 32] scores, for the weights
   void *ws;
   size_t ws_bytes;
   size_t *ws_query;

@@ -47,8 +47,8 @@ __global__ void __launch_bounds__(kWaves * 64, D <= 128 ? 2 : 1) paged_kernel(co
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);  // a scalar: units, masks and branches on them are the wave's
   const int r32 = lane & 31, g = lane >> 5;
   const int split = blockIdx.x % p.n_splits;
-  const int ct = blockIdx.x / p.n_splits % p.n_ct;
-  const int bhk = blockIdx.x / p.n_splits / p.n_ct;
+  const int tile = p.tile0 + blockIdx.x / p.n_splits;
+  const int ct = tile % p.n_ct, bhk = tile / p.n_ct;
   const int bi = bhk / p.h_k, hk = bhk % p.h_k;
   const int group = p.h / p.h_k, n_cols = group * p.sq;
   // column n = ct * 32 + r32 of the S^T tile: query head hk*group + n / sq, query row n % sq.  Its
@@ -246,7 +246,7 @@ __global__ void __launch_bounds__(kWaves * 64, D <= 128 ? 2 : 1) paged_kernel(co
     }
     if constexpr (Scores) {
       if (col_ok) {
-        float *sp = p.s_part + (((int64_t)bhk * n_cols + n) * p.max_units + j) * kUnit + g * 4;
+        float *sp = p.s_part + (((int64_t)bhk * n_cols + n - p.row0) * p.max_units + j) * kUnit + g * 4;
 #pragma unroll
         for (int i4 = 0; i4 < 4; ++i4)
           *reinterpret_cast<float4 *>(sp + i4 * 8) = float4{s[i4 * 4], s[i4 * 4 + 1], s[i4 * 4 + 2], s[i4 * 4 + 3]};
@@ -325,7 +325,7 @@ __global__ void __launch_bounds__(kWaves * 64, D <= 128 ? 2 : 1) paged_kernel(co
   const bool empty = l_all == 0.f;
   const float inv = final_pass ? (empty ? 1.f : 1.f / l_all) : 1.f;
   T *og = static_cast<T *>(p.o) + bi * p.o_bs + (int64_t)oi * p.o_rs + oh * p.o_hs;
-  const int64_t prow = (((int64_t)split * p.b + bi) * p.h + oh) * p.sq + oi;
+  const int64_t prow = split * p.n_rows + ((int64_t)bi * p.h + oh) * p.sq + oi - p.row0;
 #pragma unroll
   for (int x = 0; x < D / 8; x += 4) {
     const int dcol = slice * (D / 8) + x;
@@ -355,8 +355,9 @@ __global__ void __launch_bounds__(256) join_kernel(const PagedParams p, int grou
   __shared__ float4 acc_s[256];
   __shared__ float l_s[SETS];
   const int tid = threadIdx.x, set = tid / TPR, col = tid % TPR * 4;
-  const int64_t rows = (int64_t)p.b * p.h * p.sq;
-  const int64_t row = (int64_t)blockIdx.x * (SETS / groups) + set / groups, r = row < rows ? row : rows - 1;  // (sequence * h + head) * sq + query row
+  const int64_t rows = p.n_rows;
+  const int64_t row = (int64_t)blockIdx.x * (SETS / groups) + set / groups, at = row < rows ? row : rows - 1;  // of the launch's
+  const int64_t r = p.row0 + at;  // (sequence * h + head) * sq + query row
   const int share = set % groups;
   const int qi = (int)(r % p.sq), hq = (int)(r / p.sq % p.h), bi = (int)(r / p.sq / p.h);
   int n_live = live;
@@ -364,8 +365,8 @@ __global__ void __launch_bounds__(256) join_kernel(const PagedParams p, int grou
     const int n_units = min(p.units(p.keys_of(bi), (hq % (p.h / p.h_k) * p.sq + qi) / 32).n, p.max_units), per = p.per_split(n_units);
     n_live = max(1, (n_units + per - 1) / per);
   }
-  const float2 *ml = reinterpret_cast<const float2 *>(p.ml_part) + r;
-  const float *op = p.o_part + r * D + col;
+  const float2 *ml = reinterpret_cast<const float2 *>(p.ml_part) + at;
+  const float *op = p.o_part + at * D + col;
   float m_all = -INFINITY;
 #pragma unroll 8
   for (int s = 0; s < n_live; ++s) m_all = fmaxf(m_all, ml[s * rows].x);
@@ -398,13 +399,13 @@ __global__ void __launch_bounds__(256) join_kernel(const PagedParams p, int grou
   if (col < p.d)
     *reinterpret_cast<vec4 *>(static_cast<T *>(p.o) + bi * p.o_bs + (int64_t)qi * p.o_rs + hq * p.o_hs + col) =
         vec4{(T)(t.x * inv), (T)(t.y * inv), (T)(t.z * inv), (T)(t.w * inv)};
-  if (col == 0) p.lse[row] = empty ? INFINITY : m_all * p.scale + log2_fast(l) * kLn2;
+  if (col == 0) p.lse[r] = empty ? INFINITY : m_all * p.scale + log2_fast(l) * kLn2;
 }
 
 template <typename T, int D>
 hipError_t join_td(const PagedParams &p, int live, hipStream_t stream) {
   constexpr int SETS = 256 / (D / 4);
-  const int64_t rows = (int64_t)p.b * p.h * p.sq;
+  const int64_t rows = p.n_rows;
   int groups = 1;  // more as long as every CU has a workgroup's rows less than once
   while (groups < SETS && groups < p.n_splits && rows * groups < 256 * SETS) groups *= 2;
   const int per = SETS / groups;
@@ -414,25 +415,28 @@ hipError_t join_td(const PagedParams &p, int live, hipStream_t stream) {
 
 // weights_out[key] = weights_in[key] (0 for a row appended by this call) + sum of P over the columns of
 // the key/value head, in column order; a thread per 4 keys (of one unit), keys behind the last one
-// are left alone
-__global__ void __launch_bounds__(256) paged_weights_kernel(const PagedParams p) {
+// are left alone.  A launch of some of a key/value head's tiles goes on from the sums of those before it.
+__global__ void __launch_bounds__(256) paged_weights_kernel(const PagedParams p, int bhk0) {
   const int cap = p.pages.capacity(), blocks = (cap + 1023) / 1024;
-  const int bhk = blockIdx.x / blocks, bi = bhk / p.h_k, hk = bhk % p.h_k;
+  const int bhk = bhk0 + blockIdx.x / blocks, bi = bhk / p.h_k, hk = bhk % p.h_k;
   const int key = (blockIdx.x % blocks * 256 + threadIdx.x) * 4, sk = p.keys_of(bi);
   if (key >= sk) return;
   const int group = p.h / p.h_k, n_cols = group * p.sq, tile = key / kUnit, old = p.seqlens[bi];
   const int64_t at = (int64_t)bhk * cap + key;
   const int n = min(4, sk - key);
+  const int ct0 = max(0, p.tile0 - bhk * p.n_ct), ct1 = min(p.n_ct, p.tile0 + p.n_tiles - bhk * p.n_ct);
+  const float *w_in = ct0 > 0 ? p.w_out : p.w_in;
+  const int n_in = ct0 > 0 ? sk : w_in ? old : 0;  // rows whose weight does not start from zero
   float w[4];
 #pragma unroll
-  for (int y = 0; y < 4; ++y) w[y] = p.w_in && y < n && key + y < old ? p.w_in[at + y] : 0.f;
+  for (int y = 0; y < 4; ++y) w[y] = y < n && key + y < n_in ? w_in[at + y] : 0.f;
   const float *lse = p.lse + ((int64_t)bi * p.h + hk * group) * p.sq;  // column n's at n
-  for (int ct = 0; ct < p.n_ct; ++ct) {
+  for (int ct = ct0; ct < ct1; ++ct) {
     const idx::SinkTiles st = p.units(sk, ct);
     const int j = tile < st.ns ? tile : tile - st.n0 + st.ns;  // the unit that holds the keys
     if ((tile >= st.ns && tile < st.n0) || j >= min(st.n, p.max_units)) continue;
     const int c1 = min(n_cols, (ct + 1) * 32);
-    const float *sp = p.s_part + ((int64_t)bhk * n_cols * p.max_units + j) * kUnit + key % kUnit;
+    const float *sp = p.s_part + (((int64_t)bhk * n_cols - p.row0) * p.max_units + j) * kUnit + key % kUnit;
 #pragma unroll 4
     for (int c = ct * 32; c < c1; ++c) {
       const float4 s = *reinterpret_cast<const float4 *>(sp + (int64_t)c * p.max_units * kUnit);
@@ -449,8 +453,9 @@ __global__ void __launch_bounds__(256) paged_weights_kernel(const PagedParams p)
     if (y < n) p.w_out[at + y] = w[y];
 }
 
-hipError_t launch_weights(const PagedParams &p, hipStream_t stream) {
-  FA_LAUNCH((paged_weights_kernel), dim3((unsigned)((int64_t)((p.pages.capacity() + 1023) / 1024) * p.b * p.h_k)), dim3(256), stream, p);
+// the weights of key/value heads (sequence * h_k + head) bhk0 .. bhk1 - 1
+hipError_t launch_weights(const PagedParams &p, int bhk0, int bhk1, hipStream_t stream) {
+  FA_LAUNCH((paged_weights_kernel), dim3((unsigned)((int64_t)((p.pages.capacity() + 1023) / 1024) * (bhk1 - bhk0))), dim3(256), stream, p, bhk0);
   return hipGetLastError();
 }
 
@@ -475,30 +480,43 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const PagedParams p) 
   *reinterpret_cast<uint4 *>(vd) = *reinterpret_cast<const uint4 *>(vs);
 }
 
+// Scratch for the scores of one launch at most (one column tile's at least): a call that would take more is
+// computed in several launches, one after the other in the same scratch.  Its size follows from the
+// cache's capacity, which the host knows, and not from the lengths, which it does not.
+// Measured where it takes four launches in place of one with 1 GiB, 32 heads on 8, D = 128: 64
+// sequences in a cache of 131072 rows, one row each, 300 / 4096 / 32768 keys: 512 / 1626 / 2174 us against
+// 480 / 1708 / 2209; 8 sequences of 32768 keys, 32 rows each: 1028 against 1168.
+constexpr int64_t kScoreBytes = int64_t(256) << 20;
+
+int tile_rows(const PagedParams &p) { return std::min(32, p.h / p.h_k * p.sq); }  // most rows of a column tile
+
 template <typename T, int D>
 hipError_t paged_td(PagedParams &p, hipStream_t stream) {
-  const int64_t rows = (int64_t)p.b * p.h * p.sq;
-  const size_t s_bytes = p.w_out ? (size_t)p.b * p.h_k * (p.h / p.h_k) * p.sq * p.max_units * kUnit * sizeof(float) : 0;
-  const size_t o_bytes = p.n_splits > 1 ? (size_t)p.n_splits * rows * (D + 2) * sizeof(float) : 0;
-  const size_t need = s_bytes + o_bytes;
+  const int n_cols = p.h / p.h_k * p.sq;
+  const int64_t rows = (int64_t)p.b * p.h * p.sq, tiles = (int64_t)p.b * p.h_k * p.n_ct;
+  int64_t part = p.n_tiles;  // tiles of a launch
+  size_t s_bytes = 0, need = 0;
+  auto plan = [&]() {
+    const size_t n = (size_t)std::min(rows, part * tile_rows(p));
+    s_bytes = p.w_out ? n * p.max_units * kUnit * sizeof(float) : 0;
+    need = s_bytes + (p.n_splits > 1 ? p.n_splits * n * (D + 2) * sizeof(float) : 0);
+  };
+  plan();
   if (p.ws_query) { *p.ws_query = need; return hipSuccess; }
+  const size_t given = p.ws && (reinterpret_cast<uintptr_t>(p.ws) & 15) == 0 ? p.ws_bytes : 0;
   void *ws = nullptr;
   bool owned = false;
-  if (need) {
-    if (p.ws && (reinterpret_cast<uintptr_t>(p.ws) & 15) == 0 && p.ws_bytes >= need) ws = p.ws;
-    else if (const hipError_t e = hipMallocAsync(&ws, need, stream)) {
-      (void)hipGetLastError();
-      if (s_bytes) return e;  // the scores have nowhere to go
-      ws = nullptr;
-    } else owned = true;
-    if (!ws) p.n_splits = 1;
-    else {
-      p.s_part = s_bytes ? static_cast<float *>(ws) : nullptr;
-      if (o_bytes) {
-        p.o_part = static_cast<float *>(ws) + s_bytes / sizeof(float);
-        p.ml_part = p.o_part + (size_t)p.n_splits * rows * D;
-      }
-    }
+  while (need) {
+    if (given >= need) { ws = p.ws; break; }
+    const hipError_t e = hipMallocAsync(&ws, need, stream);
+    if (e == hipSuccess) { owned = true; break; }
+    // no memory: one split, then ever fewer tiles a launch, in the caller's scratch if that holds them
+    (void)hipGetLastError();
+    ws = nullptr;
+    if (p.n_splits > 1) p.n_splits = 1;
+    else if (part > 1) part = (part + 1) / 2;
+    else return e;  // the scores of one tile have nowhere to go
+    plan();
   }
   hipError_t e = hipSuccess;
   if (p.n_new > 0 && !p.fuse_append) {
@@ -506,16 +524,25 @@ hipError_t paged_td(PagedParams &p, hipStream_t stream) {
     FA_LAUNCH((paged_append_kernel), dim3((unsigned)((n + 255) / 256)), dim3(256), stream, p);
     e = hipGetLastError();
   }
-  const dim3 grid((unsigned)((int64_t)p.b * p.h_k * p.n_ct * p.n_splits));
-  if (e == hipSuccess) {
+  auto first_row = [&](int64_t tile) { return tile / p.n_ct * n_cols + tile % p.n_ct * 32; };
+  for (int64_t t0 = 0; t0 < tiles && e == hipSuccess; t0 += part) {
+    const int64_t t1 = std::min(tiles, t0 + part);
+    p.tile0 = (int)t0;
+    p.n_tiles = (int)(t1 - t0);
+    p.row0 = first_row(t0);
+    p.n_rows = first_row(t1) - p.row0;
+    p.s_part = s_bytes ? static_cast<float *>(ws) : nullptr;
+    if (p.n_splits > 1) {
+      p.o_part = static_cast<float *>(ws) + s_bytes / sizeof(float);
+      p.ml_part = p.o_part + p.n_splits * p.n_rows * D;
+    }
+    const dim3 grid((unsigned)(p.n_tiles * p.n_splits));
     if (p.w_out) FA_LAUNCH((paged_kernel<T, D, true>), grid, dim3(kWaves * 64), stream, p);
     else FA_LAUNCH((paged_kernel<T, D, false>), grid, dim3(kWaves * 64), stream, p);
     e = hipGetLastError();
+    if (e == hipSuccess && p.n_splits > 1) e = join_td<T, D>(p, 0, stream);
+    if (e == hipSuccess && p.w_out) e = launch_weights(p, (int)(t0 / p.n_ct), (int)((t1 + p.n_ct - 1) / p.n_ct), stream);
   }
-  if (e == hipSuccess && p.o_part) {
-    e = join_td<T, D>(p, 0, stream);
-  }
-  if (e == hipSuccess && p.w_out) e = launch_weights(p, stream);
   if (owned) {
     const hipError_t f = hipFreeAsync(ws, stream);
     if (e == hipSuccess) e = f;
@@ -536,13 +563,20 @@ hipError_t paged_t(PagedParams &p, hipStream_t stream) {
 hipError_t launch_paged(PagedParams &p, int dtype, hipStream_t stream) {
   const int cap = p.pages.capacity();
   p.n_ct = (p.h / p.h_k * p.sq + 31) / 32;
-  if (p.sq == 0) return launch_weights(p, stream);  // no columns: weights_out = weights, or zero
+  if (p.sq == 0) return launch_weights(p, 0, p.b * p.h_k, stream);  // no columns: weights_out = weights, or zero
   // most units a tile visits: the sinks' and those of a window over its rows, or the whole cache
   int64_t units = (cap + kUnit - 1) / kUnit;
   if (p.wl >= 0)
     units = std::min<int64_t>(units, (std::min(p.n_sink, cap) + kUnit - 1) / kUnit + ((int64_t)p.wl + p.sq + kUnit) / kUnit + 2);
   p.max_units = (int)std::max<int64_t>(units, 1);
-  const int64_t base = (int64_t)p.b * p.h_k * p.n_ct;
+  const int64_t tiles = (int64_t)p.b * p.h_k * p.n_ct;
+  int64_t base = tiles;  // tiles of a launch
+  if (p.w_out) {
+    const int64_t most = std::max<int64_t>(1, kScoreBytes / ((int64_t)tile_rows(p) * p.max_units * kUnit * (int)sizeof(float)));
+    const int64_t launches = (tiles + most - 1) / most;
+    base = (tiles + launches - 1) / launches;
+  }
+  p.n_tiles = (int)base;
   // Splits: one round of workgroups (two for every CU) when the sequences are few, of 128 keys (a unit
   // a wave) at least; 2048 keys each when they are many, so that unequal lengths even out.  Units
   // per split 16 / 32 / 64 / 128, kernel time: 64 x 8192 keys, 8 heads, D = 128: 368 / 351 / 346 /
@@ -568,6 +602,7 @@ hipError_t launch_sink_join(const Params &p, int width, int dtype, hipStream_t s
   a.b = p.b; a.h = p.h; a.h_k = p.h_k; a.d = p.d; a.sq = p.sq;
   a.scale = p.scale; a.scale_log2 = p.scale_log2;
   a.n_splits = p.n_splits;
+  a.n_rows = (int64_t)p.b * p.h * p.sq;
   a.o_part = p.o_part; a.ml_part = p.ml_part;
   auto go = [&](auto t) {
     using T = decltype(t);

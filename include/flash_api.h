@@ -170,7 +170,10 @@ int flash_attn_fwd_ws(void **tensors, const void *extra_args, int dtype, void *w
 int flash_attn_bwd_ws(void **tensors, const void *extra_args, int dtype, void *workspace, size_t workspace_bytes, void *stream);
 int flash_attn_kvcache_ws(void **tensors, const void *extra_args, int dtype, void *workspace, size_t workspace_bytes, void *stream);
 /* the bounded-cache calls: partials of a key split; partial dK / dV and those of the sinks; partials and
- * the scores behind the weights; nothing */
+ * the scores behind the weights; nothing.  The scores take 4 bytes a query row, head and row of the cache's
+ * capacity (of the window, where that is shorter), at most 256 MiB, or what 32 rows take where that is
+ * more: a call whose scores are more is computed in several launches, one after the other.  Where the
+ * memory cannot be had, the number of launches grows, down to 32 rows in each. */
 size_t flash_attn_sink_fwd_workspace_bytes(const void *extra_args, int dtype);
 size_t flash_attn_sink_bwd_workspace_bytes(const void *extra_args, int dtype, size_t dq_accum_bytes);
 size_t flash_attn_paged_workspace_bytes(const void *extra_args, int dtype);

@@ -1,6 +1,8 @@
 """The bounded-cache calls at the limits of what they take: windows beyond 32 bits, calls without query rows,
 scratch that is short, launches beyond what 32 bits count.  Executed on the host (emu_util)."""
 import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -67,3 +69,91 @@ def test_no_query_rows_keep_the_weights(paged, mode):
         assert torch.equal(out, want)
     need = E.workspace_bytes("paged", ops.pack_flash_paged_args(q, k, k, None, None, o, 0.2, (-1, 0), 0, n if paged else 0, mode), q.dtype)
     assert need == 0
+
+
+# The scores behind the weights are kept for 256 MiB of rows x capacity at a time, one column tile (32 rows) at least.
+SCORES = 256 << 20
+
+
+def long_cache(gen, b, hk, d, cap, page, dtype=torch.float16):
+    """A cache that could hold `cap` rows a sequence, of which the first two pages exist."""
+    n = cap // page
+    k, v = randn(gen, 2 * b, page, hk, d, dtype=dtype), randn(gen, 2 * b, page, hk, d, dtype=dtype)
+    table = torch.full((b, n), -1, dtype=torch.int32)
+    table[:, :2] = torch.randperm(2 * b, generator=gen).to(torch.int32).view(b, 2)
+    return k, v, table
+
+
+def weighted(gen, b, sq, h, hk, d, cap, n_new, lens, window, n_sink, room, page=1 << 7):
+    """A call with weights in `room(bytes asked for)` bytes of scratch (None: the library allocates) against the definition."""
+    k, v, table = long_cache(gen, b, hk, d, cap, page)
+    q = randn(gen, b, sq, h, d)
+    kn, vn = (randn(gen, b, n_new, hk, d), randn(gen, b, n_new, hk, d)) if n_new else (None, None)
+    n = torch.tensor(lens, dtype=torch.int32)
+    # the rows in use and some behind them; the rest of a long row of weights is never looked at
+    w, out = torch.rand(b, hk, cap, generator=gen), torch.full((b, hk, cap), -7.0)
+    short = 2 * page
+    want = R.paged(q, k, v, table[:, :2].contiguous(), n, 0.2, window, n_sink, kn, vn, w[:, :, :short].contiguous(), out[:, :, :short].contiguous())
+    need = E.workspace_bytes("paged", ops.pack_flash_paged_args(q, k, v, kn, vn, q, 0.2, window, n_sink, table.shape[1], 2), q.dtype)
+    ws = None if room is None else E.guarded((room(need),), torch.uint8)
+    o, lse = E.paged(q, k, v, table, n, 0.2, window, n_sink, kn, vn, w, out, workspace=ws)
+    R.close(o, want["o"], want["o_tol"], "o")
+    R.close(lse, want["lse"], want["lse_tol"], "lse")
+    R.close(out[:, :, :short], want["weights"], want["weights_tol"], "weights")
+    assert bool((out[:, :, short:] == -7).all())
+    assert torch.equal(k, want["k_pages"]) and torch.equal(v, want["v_pages"])
+    return need
+
+
+@pytest.mark.parametrize("b, sq, h, hk, cap, n_new, lens, window, n_sink", [
+    # launches that end inside a key/value head: tiles 0 1 | 2, 0 | 1 2 of 96 columns
+    (1, 24, 8, 2, 1 << 20, 24, [70], (-1, 0), 0),
+    # a tile a launch, the second of eight columns
+    (1, 40, 1, 1, 1 << 22, 0, [100], (-1, 0), 0),
+    # several sequences a launch, the new rows written by the attention itself
+    (3, 1, 8, 1, 1 << 22, 1, [200, -1, 33], (-1, 0), 0),
+])
+def test_scores_that_do_not_fit_the_scratch_at_once(b, sq, h, hk, cap, n_new, lens, window, n_sink):
+    gen = torch.Generator().manual_seed(sq)
+    need = weighted(gen, b, sq, h, hk, 32, cap, n_new, lens, window, n_sink, lambda n: n)  # exactly what was asked for
+    rows, tile = b * h * sq, min(32, h // hk * sq)
+    assert rows * cap * 4 > SCORES
+    at_once = max(tile, SCORES // (cap * 4))  # rows of a launch
+    assert need <= at_once * cap * 4 + 64 * at_once * (32 + 2) * 4  # scores, and the partials of 64 splits
+
+
+def test_without_memory_ever_fewer_tiles_a_launch():
+    """A process that may not allocate what a call asks for: the call falls back to fewer tiles a launch, in the caller's
+    scratch when that holds one, and fails with an error when there is no room for one."""
+    code = """if True:
+        import os, resource, sys
+        sys.path[:0] = [%r, %r]
+        import torch
+        torch.set_num_threads(1)
+        import test_bounded_cache_limits as T
+        import emu_util as E
+        gen = torch.Generator().manual_seed(7)
+        args = (1, 24, 8, 2, 32, 1 << 18, 24, [70], (-1, 0), 0)
+        need = T.weighted(gen, *args, None)             # everything allocated once
+        tile = 32 * (1 << 18) * 4                       # scores of one column tile: 32 MiB
+        assert need > 5 * tile
+        tight = lambda: resource.setrlimit(resource.RLIMIT_AS, (int(open("/proc/self/statm").read().split()[0]) * 4096 + room, -1))
+        paged = E.paged
+        for room, ws in ((3 * tile, None), (tile // 2, tile), (tile // 2, 2 * tile + 512)):
+            def limited(*a, **k):
+                tight()
+                try:
+                    return paged(*a, **k)
+                finally:
+                    resource.setrlimit(resource.RLIMIT_AS, (-1, -1))
+            E.paged = limited
+            T.weighted(gen, *args, None if ws is None else lambda n: ws)
+        room = tile // 2
+        try:
+            T.weighted(gen, *args, None)
+        except E.EmuFault as e:
+            assert "rc 2" in str(e), e                  # out of memory
+            print("ok without memory")
+    """ % (E.ROOT, os.path.join(E.ROOT, "tests"))
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=600)
+    assert r.returncode == 0 and "ok without memory" in r.stdout, r.stdout[-2000:] + r.stderr[-4000:]

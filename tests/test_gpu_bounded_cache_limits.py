@@ -41,3 +41,28 @@ def test_no_query_rows_keep_the_weights(paged):
     ops.flash_attn_paged(randn(g, b, 0, 4, 64), k, k, table, lens, 0.125, weights_out=out)
     want[0, :, :1500], want[2] = 0, 0
     assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("b, sq, h, hk, n_new, lens", [
+    (12, 1, 16, 4, 1, [300, 1, -1, 77, 1000, 0, 1023, 512, 31, 32, 33, 900]),  # 768 MiB of scores, several sequences a launch
+    (2, 24, 8, 2, 0, [700, 20]),                                               # tiles of a head in two launches
+])
+def test_scores_that_do_not_fit_the_scratch_at_once(b, sq, h, hk, n_new, lens):
+    g = gen(b)
+    cap, page, d, short = 1 << 20, 512, 64, 1024
+    k, v = randn(g, 2 * b, page, hk, d), randn(g, 2 * b, page, hk, d)
+    table = torch.full((b, cap // page), -1, dtype=torch.int32, device="cuda")
+    table[:, :2] = torch.randperm(2 * b, generator=g, device="cuda").to(torch.int32).view(b, 2)
+    q = randn(g, b, sq, h, d)
+    kn, vn = (randn(g, b, n_new, hk, d), randn(g, b, n_new, hk, d)) if n_new else (None, None)
+    n = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    w, out = torch.rand(b, hk, cap, generator=g, device="cuda"), torch.full((b, hk, cap), -7.0, device="cuda")
+    need = ops.flash_attn_workspace_bytes("paged", q.dtype, ops.pack_flash_paged_args(q, k, v, kn, vn, q, 0.125, (-1, 0), 0, cap // page, 2))
+    assert b * h * sq * cap * 4 > 384 << 20 and need < 272 << 20
+    want = R.paged(q, k, v, table[:, :2].contiguous(), n, 0.125, (-1, 0), 0, kn, vn, w[:, :, :short].contiguous(), out[:, :, :short].contiguous())
+    o, lse, _ = ops.flash_attn_paged(q, k, v, table, n, 0.125, k_new=kn, v_new=vn, weights=w, weights_out=out)
+    R.close(o, want["o"], want["o_tol"], "o")
+    R.close(lse, want["lse"], want["lse_tol"], "lse")
+    R.close(out[:, :, :short], want["weights"], want["weights_tol"], "weights")
+    assert bool((out[:, :, short:] == -7).all())
+    assert torch.equal(k, want["k_pages"]) and torch.equal(v, want["v_pages"])
