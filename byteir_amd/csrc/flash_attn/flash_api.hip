@@ -397,7 +397,8 @@ int evict_impl(void **tensors, const void *extra_args, int dtype, const Scratch 
   if (budget <= 0 || budget > p.to.capacity()) return fail("budget %ld does not fit the output cache (%d rows a sequence)", (long)budget, p.to.capacity());
   if (n_sink < 0 || n_recent < 0 || n_sink > budget || n_recent > budget - n_sink)
     return fail("n_sink %ld and n_recent %ld do not fit the budget %ld", (long)n_sink, (long)n_recent, (long)budget);
-  if (b * h_k > (1ll << 31) / (budget * (d / 8 + 1))) return fail("problem too large for 32-bit tile indices");
+  // the threads of a launch are counted in 32 bits: 1024 a head, and in place a column slice (below)
+  if (b * h_k > (1ll << 31) / (budget * (d / 8 + 1)) || b * h_k >= (1 << 22)) return fail("problem too large for 32-bit tile indices");
   if (sc.query) { *sc.query = 0; return 0; }
   if (b == 0) return 0;
   p.from.k_ps = st[0]; p.from.v_ps = st[1]; p.to.k_ps = st[2]; p.to.v_ps = st[3];
@@ -424,6 +425,7 @@ int evict_impl(void **tensors, const void *extra_args, int dtype, const Scratch 
   const bool same_layout = st[0] == st[2] && st[1] == st[3] && st[4] == st[6] && st[5] == st[7] && st[8] == st[10] && st[9] == st[11] && np == np_out &&
                            page == page_out && mp == mp_out && p.from.table == p.to.table;
   if (k_same != v_same || (p.in_place && !same_layout)) return fail("in place, k_out, v_out and the output table must be the cache's own");
+  if (p.in_place && b * h_k * fa::evict_groups((int)d) >= (1 << 22)) return fail("problem too large for 32-bit tile indices");
   if (p.w == p.w_out && !p.in_place) return fail("weights can be moved in place only together with the caches");
   return fa::launch_evict(p, static_cast<hipStream_t>(stream));
 }

@@ -233,8 +233,8 @@ hipError_t launch_evict(const EvictParams &p, hipStream_t stream) {
   else FA_LAUNCH((evict_select_kernel<false>), dim3((unsigned)bhk), dim3(kSelThreads), stream, p);
   if (hipError_t e = hipGetLastError()) return e;
   if (p.in_place) {
-    const int cols = 4, n_slices = (p.d / 8 + cols - 1) / cols;
-    FA_LAUNCH((evict_in_place_kernel), dim3((unsigned)(bhk * (2 * n_slices + 1))), dim3(1024), stream, p, n_slices, cols);
+    const int groups = evict_groups(p.d);
+    FA_LAUNCH((evict_in_place_kernel), dim3((unsigned)(bhk * groups)), dim3(1024), stream, p, (groups - 1) / 2, kEvictCols);
   } else {
     const int64_t n = bhk * p.budget * (p.d / 8 + 1);
     FA_LAUNCH((evict_move_kernel), dim3((unsigned)((n + 255) / 256)), dim3(256), stream, p);

@@ -98,6 +98,10 @@ struct EvictParams {
   int b, h_k, d, budget, n_sink, n_recent;
   int in_place;              // the caches are the same memory
 };
+// in place: workgroups (of 1024 threads) of one (sequence, head): slices of kEvictCols 16-byte columns of K and of
+// V, and the weights
+constexpr int kEvictCols = 4;
+inline int evict_groups(int d) { return 2 * ((d / 8 + kEvictCols - 1) / kEvictCols) + 1; }
 hipError_t launch_evict(const EvictParams &p, hipStream_t stream);
 
 }  // namespace fa

@@ -1,6 +1,7 @@
 """The bounded-cache calls at the limits of what they take: windows beyond 32 bits, calls without query rows,
 scratch that is short, launches beyond what 32 bits count.  Executed on the host (emu_util)."""
 import os
+import struct
 import subprocess
 import sys
 
@@ -157,3 +158,19 @@ def test_without_memory_ever_fewer_tiles_a_launch():
     """ % (E.ROOT, os.path.join(E.ROOT, "tests"))
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=600)
     assert r.returncode == 0 and "ok without memory" in r.stdout, r.stdout[-2000:] + r.stderr[-4000:]
+
+
+def test_evictions_beyond_a_launch_are_refused():
+    """A launch counts its threads in 32 bits, an eviction takes 1024 for a head, and in place for a column slice of one:
+    more are refused before anything is launched."""
+    def blob(b, hk, d, page=2):  # a dense cache, in place
+        return struct.pack("<24q", *[d] * 12, b, hk, d, b, page, 0, b, page, 0, 1, 0, 0)
+    # never looked at: one tensor stands for them all
+    t, n = torch.zeros(16, dtype=torch.float16), torch.zeros(16, dtype=torch.int32)
+    w = torch.zeros(16)
+    other = torch.zeros(16, dtype=torch.float16)
+    for b, hk, d in ((1 << 22, 1, 8), (1 << 12, 1 << 10, 8), (1 << 12, 64, 256), (1 << 20, 2, 8)):
+        with pytest.raises(E.EmuFault, match="too large"):
+            E._call("evict", [t, t, w, n, None, t, t, None, w, n, n], blob(b, hk, d), torch.float16)
+    with pytest.raises(E.EmuFault, match="too large"):  # into another cache
+        E._call("evict", [t, t, w, n, None, other, other, None, w.clone(), n, n], blob(1 << 22, 1, 8), torch.float16)
