@@ -405,6 +405,8 @@ def _launch(plan, tensors, on, workspace):
     if workspace is not None:
         if workspace.get_device() != device:
             raise ValueError("the workspace must lie on the tensors' GPU")
+        if not workspace.is_contiguous():  # its bytes are counted by its elements
+            raise ValueError("the workspace must be dense")
         ws, n = workspace.data_ptr(), workspace.numel() * workspace.element_size()
     elif need:
         workspace = torch.empty(need, dtype=torch.uint8, device=on.device)

@@ -174,3 +174,12 @@ def test_evictions_beyond_a_launch_are_refused():
             E._call("evict", [t, t, w, n, None, t, t, None, w, n, n], blob(b, hk, d), torch.float16)
     with pytest.raises(E.EmuFault, match="too large"):  # into another cache
         E._call("evict", [t, t, w, n, None, other, other, None, w.clone(), n, n], blob(1 << 22, 1, 8), torch.float16)
+
+
+def test_a_broadcast_workspace_is_refused(monkeypatch):
+    """Its elements say nothing of the bytes behind it."""
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: -1)  # where CPU tensors say they lie
+    plan = (lambda *a: pytest.fail("launched"), b"", 1, 1 << 20)
+    for ws in (torch.zeros(1, dtype=torch.uint8).expand(1 << 20), torch.zeros(1 << 21, dtype=torch.uint8)[::2]):
+        with pytest.raises(ValueError, match="workspace must be dense"):
+            ops._launch(plan, b"", torch.zeros(1), ws)
