@@ -567,6 +567,9 @@ __global__ void __launch_bounds__(256, DR <= 64 ? 2 : 1) dkdv_anyd_kernel(const 
 // own and those of P in P V).  With e = sum_j P (dP - D), which would be zero for the D of these P
 // and dP, D + e has none of them; dQ is corrected by -e scale sum_j P K (one more product that shares
 // the K fragments of dS K), and D + e is written for the dK / dV kernel.  With d_rows only D + e is wanted.
+// The second set of sums costs registers: from 128 columns on they spill (44, 664 and 1424 bytes a lane at
+// 128, 192 and 256; without Exact, none).  2 x 2048 rows, 16 heads, window 256: 72, 85, 190 and 339 us
+// at d = 96, 128, 192 and 256; the plain form takes 68, 74, 178 and 221 for a window of 1024.
 template <typename T, int DR, bool Drop, bool Sink = false, bool Exact = false>
 __global__ void __launch_bounds__(256, (Exact ? DR <= 64 : DR <= 96 || (DR == 128 && !Drop)) ? 2 : 1) dq_anyd_kernel(const Params p) {
   using vec8 = typename Traits<T>::vec8;

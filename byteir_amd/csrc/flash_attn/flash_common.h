@@ -321,13 +321,13 @@ bool sink_few_rows(const Params &p);
 // joins p.n_splits partials with rows of `width` floats into p.o_w and p.lse
 hipError_t launch_sink_join(const Params &p, int width, int dtype, hipStream_t stream);
 hipError_t launch_sink_few_rows(const Params &p, int dtype, hipStream_t stream);
-// most key tiles of `bn` rows that a block of `bm` query rows of a flash_attn_sink_fwd call visits
 // log2 of the query heads of a key/value head that can share a workgroup of `waves` waves
 inline int head_pack(const Params &p, int waves) {
   int n = 0;
   while ((2 << n) <= waves && p.h / p.h_k % (2 << n) == 0) ++n;
   return n;
 }
+// most key tiles of `bn` rows that a block of `bm` query rows of a flash_attn_sink_fwd call visits
 inline int sink_tiles_bound(const Params &p, int bm, int bn) {
   const int all = (p.sk + bn - 1) / bn;
   if (p.wl < 0 || p.wr < 0) return all;

@@ -44,7 +44,8 @@ constexpr float kRescaleSlack = 8.0f;
 // query heads of one key/value head share a workgroup: its waves take their heads in turn and
 // the block has that many times fewer rows, so that its tiles span the window and little more
 // (32 heads on 8, window 1024: 18 tiles and the sinks' for 64 rows of four heads against 21 for 256
-// of one; D = 128, 8192 rows: 210 us against 231).
+// of one; D = 128, 8192 rows: 210 us against 231 in the first forty launches after a pause, 175 in a
+// long run, when the clock has risen).
 template <typename T, int D, int QB, int NW, bool VarK, bool Sink = false>
 __global__ void __launch_bounds__(NW * 64, NW * QB >= 16 ? 2 : (QB == 2 ? 1 : 2)) flash_fwd_kernel(const Params p) {
   constexpr int kThreads = NW * 64;

@@ -11,14 +11,17 @@
 // LDS tiles with the next unit in flight and no barrier in the loop, the waves join in LDS, the
 // workgroups that share a sequence's keys join through fp32 partials in a second kernel.
 // What differs: a unit's 32 row addresses come from the block table, looked up by one lane per row a
-// unit ahead of the loads that need them and handed round by lane permutes; the keys are cut by
+// unit ahead of the loads that need them: a scalar for the rows of one pass where the page size is a
+// multiple of their number, else handed round by lane permutes; the keys are cut by
 // the sequence's own length (units are numbered through sinks and window, and every sequence
 // shares its units out evenly over the splits the grid offers it), so a short sequence in a long
 // cache does not wait for one workgroup; rows that nobody sees (outside the window, behind the
 // last key, on an absent page) are not read and count as zeros.
 // Measured, 32 heads on 8, D = 128, fp16: 64 x 8192 keys 340 us = 6.3 TB/s; 64 x 1000..8191 keys
-// (bf16, 1.21 GB) 201 us = 6.0 TB/s; one sequence of 31 keys 8.6 us, of 300 12 us (latency: length,
-// table, rows, then 2 us a unit); 16 heads, D = 64, 64 x 8192 keys 366 us = 5.9 TB/s.
+// (bf16, 1.21 GB) 199 us = 6.0 TB/s; one sequence of 31 keys 8.6 us, of 300 12 us (latency: length,
+// table, rows, then 2 us a unit); 16 heads, D = 64, 64 x 8192 keys 366 us = 5.9 TB/s.  Above 128 columns
+// the registers do not hold a unit in flight: 80 bytes a lane spill, 148 with weights.  Every 32
+// columns (rows x query heads of a key/value head) are workgroups of their own that read the keys again.
 #include <algorithm>
 
 #include "flash_paged.h"

@@ -10,12 +10,12 @@
 // query rows) items; its waves take the items in turn, each with K, V and the accumulators of the
 // same 32 keys in registers and a private Q / dO tile in LDS (no barrier in the loop; the next
 // item's rows are in flight meanwhile).  What bounds it is reading Q and dO once per 32 sinks:
-// 4 d bytes a row against 128 d flops a row and key block of MFMA.  The waves' sums meet in LDS,
+// 4 d bytes a row against 256 d flops a row and key block of MFMA (four products of 32 keys).  The waves' sums meet in LDS,
 // the shares' as fp32 partials that sink_join_kernel adds in order: no atomics, same bits every run.
 // Without scratch there is one share and the workgroup rounds its sums itself.
-// Measured: 4 sinks, 8192 rows, 32 heads on 8, D = 128: 46-50 us (Q and dO, 134 MB, in 20 at the
+// Measured: 4 sinks, 8192 rows, 32 heads on 8, D = 128: 49 us (Q and dO, 134 MB, in 20 at the
 // rate of a read stream; four items a wave, each a memory latency); 128 sinks, 2 x 2048 rows, 16
-// heads on 2, d = 96: 26 us.  Two waves per SIMD instead of one with the next item in flight: 38 -> 25 us there.
+// heads on 2, d = 96: 25 us.  Two waves per SIMD instead of one with the next item in flight: 38 -> 25 us there.
 #include <algorithm>
 
 #include "flash_common.h"
