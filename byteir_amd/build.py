@@ -12,9 +12,11 @@ and, for the tests alone (a build of everything goes on without one that fails):
   test_kernels -> tests/external_kernels/libcustom_add.so
   emu -> tests/emu/lib/*.so               the same sources for the host
 """
+import concurrent.futures
 import os
 import subprocess
 import sys
+import tempfile
 import time
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -25,7 +27,7 @@ INC = os.path.join(ROOT, "include")
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 # -packed-fp32-ops is switched off on purpose: the compiler must not form v_pk_*_f32.
-HIP_FLAGS = ["-O3", "-std=c++17", "--offload-arch=gfx950", "-fPIC", "-shared",
+HIP_FLAGS = ["-O3", "-std=c++17", "--offload-arch=gfx950", "-fPIC",
              "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
              "-Wno-unused-command-line-argument", f"-I{INC}"]
 CXX_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", f"-I{INC}"]
@@ -48,15 +50,24 @@ def _run(cmd, verbose):
             print(out)
 
 
-def build_kernels(verbose=False):
+def _hip_library(name, srcs, flags, verbose):
+    """lib/<name> from sources compiled side by side (the attention kernels: 160 s one after the other)."""
     os.makedirs(LIB, exist_ok=True)
-    _run([HIPCC] + HIP_FLAGS + ["-o", os.path.join(LIB, "libbrt_rocm_kernels.so")] + _glob("kernels", (".hip",)), verbose)
+    t = time.time()
+    with tempfile.TemporaryDirectory() as tmp, concurrent.futures.ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as pool:
+        objs = [os.path.join(tmp, os.path.basename(src) + ".o") for src in srcs]
+        list(pool.map(lambda j: _run([HIPCC] + HIP_FLAGS + flags + ["-c", j[0], "-o", j[1]], False), zip(srcs, objs)))
+        if verbose:
+            print(f"[build] {len(srcs)} sources of {name} in {time.time() - t:.1f}s")
+        _run([HIPCC] + HIP_FLAGS + ["-shared", "-o", os.path.join(LIB, name)] + objs, verbose)
+
+
+def build_kernels(verbose=False):
+    _hip_library("libbrt_rocm_kernels.so", _glob("kernels", (".hip",)), [], verbose)
 
 
 def build_flash(verbose=False):
-    os.makedirs(LIB, exist_ok=True)
-    _run([HIPCC] + HIP_FLAGS + [f"-I{os.path.join(CSRC, 'flash_attn')}", "-o", os.path.join(LIB, "libflash_attn.so")]
-         + _glob("flash_attn", (".hip",)), verbose)
+    _hip_library("libflash_attn.so", _glob("flash_attn", (".hip",)), [f"-I{os.path.join(CSRC, 'flash_attn')}"], verbose)
 
 
 def build_brt(verbose=False):
@@ -82,7 +93,7 @@ def build_test_kernels(verbose=False):
     src = os.path.join(ROOT, "tests", "external_kernels", "custom_add.hip")
     if not os.path.exists(src):
         return
-    _run([HIPCC] + HIP_FLAGS + [f"-I{os.path.join(CSRC, 'brt')}", "-o",
+    _run([HIPCC] + HIP_FLAGS + ["-shared", f"-I{os.path.join(CSRC, 'brt')}", "-o",
                                 os.path.join(ROOT, "tests", "external_kernels", "libcustom_add.so"), src,
                                 f"-L{LIB}", "-lbrt", "-lbrt_rocm_kernels", f"-Wl,-rpath,{LIB}"], verbose)
 
@@ -99,7 +110,6 @@ def build_emu(verbose=False):
     emu = os.path.join(ROOT, "tests", "emu")
     if not os.path.exists(clang) or not os.path.isdir(emu):
         return
-    import concurrent.futures
     obj, out = os.path.join(emu, "obj"), os.path.join(emu, "lib")
     os.makedirs(obj, exist_ok=True)
     os.makedirs(out, exist_ok=True)
