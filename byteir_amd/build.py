@@ -144,17 +144,22 @@ TARGETS = {"kernels": build_kernels, "flash": build_flash, "brt": build_brt, "in
 def build_all(verbose=False, targets=None):
     """The named targets, or all.  Of all, those for the tests may fail (a tests/ directory of another age): that is
     printed, and nothing older is left in their place for a test to load."""
+    def drop(name):
+        for f in TEST_TARGETS.get(name, ()):
+            if os.path.exists(os.path.join(ROOT, f)):
+                os.remove(os.path.join(ROOT, f))
+
     for name in targets or TARGETS:
-        old = [os.path.join(ROOT, f) for f in TEST_TARGETS.get(name, ())]
-        for f in filter(os.path.exists, old):
-            os.remove(f)
         try:
+            drop(name)
             TARGETS[name](verbose)
         except Exception as e:
             if targets or name not in TEST_TARGETS:
                 raise
-            for f in filter(os.path.exists, old):
-                os.remove(f)
+            try:
+                drop(name)
+            except OSError:  # a directory that cannot be written to: nothing was built there either
+                pass
             print(f"[build] {name} (for the tests only) does not build, going on without it: {e}", file=sys.stderr)
 
 

@@ -138,7 +138,8 @@ def test_without_memory_ever_fewer_tiles_a_launch():
         need = T.weighted(gen, *args, None)             # everything allocated once
         tile = 32 * (1 << 18) * 4                       # scores of one column tile: 32 MiB
         assert need > 5 * tile
-        tight = lambda: resource.setrlimit(resource.RLIMIT_AS, (int(open("/proc/self/statm").read().split()[0]) * 4096 + room, -1))
+        soft, hard = resource.getrlimit(resource.RLIMIT_AS)
+        tight = lambda: resource.setrlimit(resource.RLIMIT_AS, (int(open("/proc/self/statm").read().split()[0]) * resource.getpagesize() + room, hard))
         paged = E.paged
         for room, ws in ((3 * tile, None), (tile // 2, tile), (tile // 2, 2 * tile + 512)):
             def limited(*a, **k):
@@ -146,7 +147,7 @@ def test_without_memory_ever_fewer_tiles_a_launch():
                 try:
                     return paged(*a, **k)
                 finally:
-                    resource.setrlimit(resource.RLIMIT_AS, (-1, -1))
+                    resource.setrlimit(resource.RLIMIT_AS, (soft, hard))
             E.paged = limited
             T.weighted(gen, *args, None if ws is None else lambda n: ws)
         room = tile // 2

@@ -38,6 +38,22 @@ def test_a_tests_directory_that_does_not_fit_stops_nothing(tmp_path, monkeypatch
             B.build_all(targets=[name])
 
 
+def test_a_tests_directory_that_cannot_be_written_to_stops_nothing(tmp_path, monkeypatch, capsys):
+    done = []
+    for name in B.TARGETS:
+        monkeypatch.setitem(B.TARGETS, name, lambda verbose, name=name: done.append(name))
+
+    def refuse(path):
+        raise PermissionError(path)
+    monkeypatch.setattr(B, "ROOT", str(tmp_path))
+    monkeypatch.setattr(B.os, "remove", refuse)
+    (tmp_path / "tests/emu/lib").mkdir(parents=True)
+    (tmp_path / B.TEST_TARGETS["emu"][0]).write_text("another user's")
+    B.build_all()
+    assert "emu (for the tests only) does not build" in capsys.readouterr().err
+    assert done == [name for name in B.TARGETS if name != "emu"]
+
+
 def test_a_product_library_that_does_not_build_stops_the_build(monkeypatch):
     def fail(verbose):
         raise RuntimeError("build failed")
