@@ -66,3 +66,41 @@ def test_scores_that_do_not_fit_the_scratch_at_once(b, sq, h, hk, n_new, lens):
     R.close(out[:, :, :short], want["weights"], want["weights_tol"], "weights")
     assert bool((out[:, :, short:] == -7).all())
     assert torch.equal(k, want["k_pages"]) and torch.equal(v, want["v_pages"])
+
+
+def test_a_call_of_several_launches_is_captured_and_replayed():
+    """Replayed three times on new inputs, with eager calls between, in scratch of its own."""
+    g = gen(3)
+    b, h, hk, d, cap, page = 12, 16, 4, 64, 1 << 20, 512
+    k, v = torch.empty(2 * b, page, hk, d, device="cuda", dtype=torch.float16), torch.empty(2 * b, page, hk, d, device="cuda", dtype=torch.float16)
+    table = torch.full((b, cap // page), -1, dtype=torch.int32, device="cuda")
+    table[:, :2] = torch.arange(2 * b, device="cuda", dtype=torch.int32).view(b, 2)
+    q, kn, vn = (torch.empty(b, 1, n, d, device="cuda", dtype=torch.float16) for n in (h, hk, hk))
+    n = torch.randint(0, 1000, (b,), generator=g, device="cuda").to(torch.int32)
+    w, out = torch.zeros(b, hk, cap, device="cuda"), torch.zeros(b, hk, cap, device="cuda")
+
+    def run():
+        return ops.flash_attn_paged(q, k, v, table, n, 0.125, k_new=kn, v_new=vn, weights=w, weights_out=out)
+
+    def fill():
+        for t in (q, k, v, kn, vn):
+            t.copy_(randn(g, *t.shape))
+        w[:, :, :1024] = torch.rand(b, hk, 1024, generator=g, device="cuda")
+
+    fill()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = run()
+    for _ in range(3):
+        fill()
+        want = [t.clone() for t in run()]
+        out.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(map(torch.equal, captured, want))
